@@ -43,7 +43,7 @@ def _load() -> C.CDLL:
 
 lib = _load()
 
-_vp, _sz, _i, _f, _u64 = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_uint64
+_vp, _sz, _i, _f, _u64, _u32 = C.c_void_p, C.c_size_t, C.c_int, C.c_float, C.c_uint64, C.c_uint32
 
 
 class AdamWTensor(C.Structure):
@@ -128,6 +128,17 @@ SIGNATURES = {
     "cgpt_swiglu_backward": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _vp]),
     "cgpt_embedding_forward": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _i, _vp]),
     "cgpt_embedding_backward": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _i, _i, _i, _vp]),
+    "cgpt_dropout_forward": (_i, [_vp, _vp, _vp, _sz, _f, _vp, _u32, _i, _vp]),
+    "cgpt_dropout_backward": (_i, [_vp, _vp, _sz, _f, _vp, _u32, _i, _i, _vp]),
+    "cgpt_dropout_advance": (_i, [_vp, _u64, _vp]),
+    "cgpt_layernorm_forward": (_i, [_vp] * 4 + [_sz, _sz, _f, _i, _vp]),
+    "cgpt_layernorm_backward_workspace_bytes": (_sz, [_sz, _sz]),
+    "cgpt_layernorm_backward": (_i, [_vp] * 8 + [_sz] * 3 + [_f, _i, _vp]),
+    "cgpt_dropout_add_layernorm_forward": (_i, [_vp] * 6 + [_sz, _sz, _f, _f, _vp, _u32, _i, _vp]),
+    "cgpt_dropout_add_layernorm_backward": (_i, [_vp] * 9 + [_sz] * 3 + [_f, _f, _vp, _u32, _i, _vp]),
+    "cgpt_scaled_embedding_forward": (_i, [_vp] * 3 + [_sz] * 3 + [_f, _f, _vp, _u32, _i, _vp]),
+    "cgpt_scaled_embedding_backward_workspace_bytes": (_sz, [_sz, _sz]),
+    "cgpt_scaled_embedding_backward": (_i, [_vp] * 4 + [_sz] * 4 + [_f, _u32, _f, _vp, _u32, _i, _i, _vp]),
     "cgpt_add": (_i, [_vp, _vp, _vp, _vp, _sz, _i, _vp]),
     "cgpt_cross_entropy": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _f, _i, _vp]),
     "cgpt_adamw_create": (_i, [C.POINTER(_vp), C.POINTER(AdamWTensor), _sz, _u64, _vp]),

@@ -1,0 +1,298 @@
+// Layer norm forward and backward, and the same fused with dropout and the residual add in front of it, for sm_100a.
+//
+//   forward    mean = sum x / H, var = sum (x - mean)^2 / H, rstd = 1 / sqrt(var + eps), y = (x - mean) rstd w + b
+//   backward   xh = (x - mean) rstd, g = dy w:   dx = rstd (g - mean(g) - xh mean(g xh)) (+ residual)
+//              dw = sum_rows dy xh,  db = sum_rows dy
+//   fused      x = residual + dropout(in), rounded to the storage type and written, then the norm of the rounded value;
+//              backward: d = dsum + dx, dresidual = d, din = dropout map of d
+//
+// The variance is taken around the mean (a second pass over values that are already on the chip): sum x^2 - mean^2 loses
+// everything for a row whose offset is large against its spread. The backward recomputes mean and rstd from x, which it reads
+// in any case, so the forward stores no statistics. Sums are fp32; a row's dw and db contributions are added in a fixed order
+// (per-CTA partial rows, then one pass over them), so results repeat bit for bit.
+//
+// Memory-bound: 2 * H * sizeof(T) bytes per row forward, 3 backward (+1 with a residual), 4 and 5 for the fused pair.
+#include "philox.cuh"
+#include "launch_counter.h"
+
+namespace cgpt {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+// Sum of `vals` over the CTA; every thread gets the totals. Contains barriers.
+template <int NV, int WARPS>
+__device__ __forceinline__ void block_sum(float (&vals)[NV], float* smem /* [WARPS * NV] */) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) vals[i] = warp_sum(vals[i]);
+    __syncthreads();   // the previous call's totals have been read
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) smem[(threadIdx.x >> 5) * NV + i] = vals[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) acc += smem[w * NV + i];
+        vals[i] = acc;
+    }
+}
+
+// The element-wise formulas, with every fused multiply-add written out: left to the compiler, the contractions differ between
+// instantiations, and the fused operators would not give the bits of their parts.
+__device__ __forceinline__ float normalised(float x, float mean, float rstd) { return __fmul_rn(x - mean, rstd); }
+__device__ __forceinline__ float norm_dx(float dy, float w, float xh, float rstd, float c1, float c2, float residual) {
+    return fmaf(rstd, fmaf(-xh, c2, fmaf(dy, w, -c1)), residual);
+}
+// sums of (x - mean)^2, g and g (x - mean) with g = dy w
+__device__ __forceinline__ void norm_sums(float (&s)[3], float dy, float w, float d) {
+    s[0] = fmaf(d, d, s[0]);
+    s[1] = fmaf(dy, w, s[1]);
+    s[2] = fmaf(__fmul_rn(dy, w), d, s[2]);
+}
+
+// ------------------------------------------------------------------------------------------ rows of any length
+// One CTA per row, the row read again (from L1/L2) for every pass over it. Any H, any alignment.
+template <typename T, bool FUSED>
+__global__ void __launch_bounds__(kThreads)
+layernorm_forward_any_kernel(T* __restrict__ y, T* sum, const T* x, const T* residual, const T* __restrict__ w,
+                             const T* __restrict__ b, long long rows, long long hidden, float epsilon, const DropoutArgs args) {
+    __shared__ float red[kWarps];
+    const Philox gen(args);
+    const float inv_hidden = 1.0f / static_cast<float>(hidden);
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* in = (FUSED ? sum : x) + row * hidden;
+        float s[1] = {0.f};
+        for (long long c = threadIdx.x; c < hidden; c += kThreads) {
+            if constexpr (FUSED) {
+                const long long e = row * hidden + c;
+                float v = to_f32<T>(x[e]);
+                if (args.threshold != 0) v = apply_one(v, gen, e, args);
+                const T stored = from_f32<T>(v + to_f32<T>(residual[e]));
+                sum[e] = stored;             // read again below by this thread only
+                s[0] += to_f32<T>(stored);
+            } else {
+                s[0] += to_f32<T>(in[c]);
+            }
+        }
+        block_sum<1, kWarps>(s, red);
+        const float mean = s[0] * inv_hidden;
+        s[0] = 0.f;
+        for (long long c = threadIdx.x; c < hidden; c += kThreads) {
+            const float d = to_f32<T>(in[c]) - mean;
+            s[0] = fmaf(d, d, s[0]);
+        }
+        block_sum<1, kWarps>(s, red);
+        const float rstd = rsqrtf(fmaf(s[0], inv_hidden, epsilon));
+        for (long long c = threadIdx.x; c < hidden; c += kThreads)
+            y[row * hidden + c] = from_f32<T>(fmaf(normalised(to_f32<T>(in[c]), mean, rstd), to_f32<T>(w[c]), b != nullptr ? to_f32<T>(b[c]) : 0.f));
+    }
+}
+
+// dx (FUSED: dresidual and din) of one row per CTA; the row's (mean, rstd) go to `stats` for the column sums.
+template <typename T, bool FUSED>
+__global__ void __launch_bounds__(kThreads)
+layernorm_backward_any_kernel(T* dx, T* din, float2* __restrict__ stats, const T* __restrict__ dy, const T* __restrict__ x,
+                              const T* __restrict__ w, const T* residual, long long rows, long long hidden, float epsilon,
+                              const DropoutArgs args) {
+    __shared__ float red[kWarps * 3];
+    const Philox gen(args);
+    const float inv_hidden = 1.0f / static_cast<float>(hidden);
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * hidden;
+        const T* gr = dy + row * hidden;
+        float m[1] = {0.f};
+        for (long long c = threadIdx.x; c < hidden; c += kThreads) m[0] += to_f32<T>(xr[c]);
+        block_sum<1, kWarps>(m, red);
+        const float mean = m[0] * inv_hidden;
+        float s[3] = {0.f, 0.f, 0.f};   // sum (x - mean)^2, sum g, sum g (x - mean)
+        for (long long c = threadIdx.x; c < hidden; c += kThreads) norm_sums(s, to_f32<T>(gr[c]), to_f32<T>(w[c]), to_f32<T>(xr[c]) - mean);
+        block_sum<3, kWarps>(s, red);
+        const float rstd = rsqrtf(fmaf(s[0], inv_hidden, epsilon));
+        const float c1 = s[1] * inv_hidden, c2 = s[2] * inv_hidden * rstd;
+        for (long long c = threadIdx.x; c < hidden; c += kThreads) {
+            const long long e = row * hidden + c;
+            const float d = norm_dx(to_f32<T>(gr[c]), to_f32<T>(w[c]), normalised(to_f32<T>(xr[c]), mean, rstd), rstd, c1, c2,
+                                    residual != nullptr ? to_f32<T>(residual[e]) : 0.f);
+            dx[e] = from_f32<T>(d);
+            if constexpr (FUSED) din[e] = from_f32<T>(args.threshold != 0 ? apply_one(d, gen, e, args) : d);
+        }
+        if (threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
+    }
+}
+
+// Column sums of dy * xh and dy over a share of the rows: 32 columns and 8 row lanes per CTA, rows split over blockIdx.y.
+// partial: [splits][2][hidden].
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+layernorm_columns_any_kernel(float* __restrict__ partial, const T* __restrict__ dy, const T* __restrict__ x,
+                             const float2* __restrict__ stats, long long rows, long long hidden) {
+    __shared__ float tile[2][kWarps][33];
+    const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const long long col = static_cast<long long>(blockIdx.x) * 32 + lane;
+    const long long share = (rows + gridDim.y - 1) / gridDim.y;
+    const long long first = blockIdx.y * share, last = first + share < rows ? first + share : rows;
+    float aw = 0.f, ab = 0.f;
+    if (col < hidden) {
+        for (long long r = first + rl; r < last; r += kWarps) {
+            const float2 st = stats[r];
+            const float g = to_f32<T>(dy[r * hidden + col]);
+            aw = fmaf(g, normalised(to_f32<T>(x[r * hidden + col]), st.x, st.y), aw);
+            ab += g;
+        }
+    }
+    tile[0][rl][lane] = aw;
+    tile[1][rl][lane] = ab;
+    __syncthreads();
+    if (rl < 2 && col < hidden) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) t += tile[rl][k][lane];
+        partial[(static_cast<long long>(blockIdx.y) * 2 + rl) * hidden + col] = t;
+    }
+}
+
+// dw and db from `parts` partial rows ([parts][2][hidden]) in a fixed order: 32 columns, 32 row lanes per CTA; blockIdx.y
+// chooses dw or db.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __restrict__ partial, int parts, long long hidden) {
+    __shared__ float tile[32][33];
+    const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const long long col = static_cast<long long>(blockIdx.x) * 32 + lane;
+    float acc = 0.f;
+    if (col < hidden)
+        for (int p = rl; p < parts; p += 32) acc += partial[(static_cast<long long>(p) * 2 + blockIdx.y) * hidden + col];
+    tile[rl][lane] = acc;
+    __syncthreads();
+    if (rl == 0 && col < hidden) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) t += tile[r][lane];
+        (blockIdx.y == 0 ? dw : db)[col] = from_f32<T>(t);
+    }
+}
+
+constexpr std::size_t kMaxSplits = 64;
+std::size_t any_splits(std::size_t rows) {
+    const std::size_t n = (rows + 63) / 64;
+    return n < kMaxSplits ? n : kMaxSplits;
+}
+
+unsigned any_grid(std::size_t rows) { return static_cast<unsigned>(rows < kNumSMs * 8ull ? rows : kNumSMs * 8ull); }
+
+bool valid_rows(std::size_t rows, std::size_t hidden) {
+    return rows != 0 && hidden != 0 && hidden <= 0x7fffffffull && rows <= (1ull << 46) / hidden;
+}
+
+std::size_t workspace_bytes(std::size_t rows, std::size_t hidden) {
+    return rows * sizeof(float2) + any_splits(rows) * 2 * hidden * sizeof(float);
+}
+
+template <typename T, bool FUSED>
+int launch_forward(void* y, void* sum, const void* x, const void* residual, const void* w, const void* b, std::size_t rows,
+                   std::size_t hidden, float epsilon, const DropoutArgs& args, cudaStream_t s) {
+    layernorm_forward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
+        static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
+        static_cast<const T*>(w), static_cast<const T*>(b), static_cast<long long>(rows), static_cast<long long>(hidden), epsilon, args);
+    count_launch();
+    CGPT_LAUNCH_CHECK();
+    return CGPT_OK;
+}
+
+template <typename T, bool FUSED>
+int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, const void* x, const void* w, const void* residual,
+                    void* workspace, std::size_t rows, std::size_t hidden, float epsilon, const DropoutArgs& args, cudaStream_t s) {
+    const std::size_t splits = any_splits(rows);
+    float* partial = static_cast<float*>(workspace);
+    float2* stats = reinterpret_cast<float2*>(partial + splits * 2 * hidden);
+    layernorm_backward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
+        static_cast<T*>(dx), static_cast<T*>(din), stats, static_cast<const T*>(dy), static_cast<const T*>(x),
+        static_cast<const T*>(w), static_cast<const T*>(residual), static_cast<long long>(rows), static_cast<long long>(hidden),
+        epsilon, args);
+    count_launch();
+    CGPT_LAUNCH_CHECK();
+    const unsigned columns = static_cast<unsigned>((hidden + 31) / 32);
+    layernorm_columns_any_kernel<T><<<dim3(columns, static_cast<unsigned>(splits)), kThreads, 0, s>>>(
+        partial, static_cast<const T*>(dy), static_cast<const T*>(x), stats, static_cast<long long>(rows), static_cast<long long>(hidden));
+    count_launch();
+    CGPT_LAUNCH_CHECK();
+    layernorm_reduce_kernel<T><<<dim3(columns, db != nullptr ? 2 : 1), 1024, 0, s>>>(
+        static_cast<T*>(dw), static_cast<T*>(db), partial, static_cast<int>(splits), static_cast<long long>(hidden));
+    count_launch();
+    CGPT_LAUNCH_CHECK();
+    return CGPT_OK;
+}
+
+}  // namespace
+}  // namespace cgpt
+
+using namespace cgpt;
+
+extern "C" int cgpt_layernorm_forward(void* y, const void* x, const void* w, const void* b, size_t rows, size_t hidden,
+                                      float epsilon, int dtype, cgpt_stream_t stream) {
+    if (!y || !x || !w) return CGPT_ERR_NULL;
+    if (!valid_float_dtype(dtype)) return CGPT_ERR_DTYPE;
+    if (!valid_rows(rows, hidden)) return CGPT_ERR_SHAPE;
+    if (!(epsilon > 0.f) || y == x) return CGPT_ERR_OPTION;
+    if (!element_aligned(dtype, {y, x, w, b})) return CGPT_ERR_ALIGN;
+    auto s = static_cast<cudaStream_t>(stream);
+    CGPT_DISPATCH_DTYPE(dtype, T, { return (launch_forward<T, false>(y, nullptr, x, nullptr, w, b, rows, hidden, epsilon, DropoutArgs{}, s)); });
+    return CGPT_OK;
+}
+
+extern "C" size_t cgpt_layernorm_backward_workspace_bytes(size_t rows, size_t hidden) {
+    return valid_rows(rows, hidden) ? workspace_bytes(rows, hidden) : 0;
+}
+
+extern "C" int cgpt_layernorm_backward(void* dx, void* dw, void* db, const void* dy, const void* x, const void* w,
+                                       const void* residual, void* workspace, size_t workspace_size, size_t rows, size_t hidden,
+                                       float epsilon, int dtype, cgpt_stream_t stream) {
+    if (!dx || !dw || !dy || !x || !w || !workspace) return CGPT_ERR_NULL;
+    if (!valid_float_dtype(dtype)) return CGPT_ERR_DTYPE;
+    if (!valid_rows(rows, hidden) || workspace_size < workspace_bytes(rows, hidden)) return CGPT_ERR_SHAPE;
+    if (!(epsilon > 0.f) || dx == dy || dx == x) return CGPT_ERR_OPTION;
+    if (!element_aligned(dtype, {dx, dw, db, dy, x, w, residual}) || !aligned16(workspace)) return CGPT_ERR_ALIGN;
+    auto s = static_cast<cudaStream_t>(stream);
+    CGPT_DISPATCH_DTYPE(dtype, T, {
+        return (launch_backward<T, false>(dx, nullptr, dw, db, dy, x, w, residual, workspace, rows, hidden, epsilon, DropoutArgs{}, s));
+    });
+    return CGPT_OK;
+}
+
+extern "C" int cgpt_dropout_add_layernorm_forward(void* y, void* sum, const void* x, const void* residual, const void* w,
+                                                  const void* b, size_t rows, size_t hidden, float epsilon, float probability,
+                                                  const uint64_t* state, uint32_t site, int dtype, cgpt_stream_t stream) {
+    if (!y || !sum || !x || !residual || !w) return CGPT_ERR_NULL;
+    if (!valid_float_dtype(dtype)) return CGPT_ERR_DTYPE;
+    if (!valid_rows(rows, hidden)) return CGPT_ERR_SHAPE;
+    if (!(epsilon > 0.f) || y == x || y == residual || y == sum) return CGPT_ERR_OPTION;
+    if (!element_aligned(dtype, {y, sum, x, residual, w, b})) return CGPT_ERR_ALIGN;
+    DropoutArgs args;
+    CGPT_TRY(dropout_args(&args, probability, state, site, rows * hidden));
+    auto s = static_cast<cudaStream_t>(stream);
+    CGPT_DISPATCH_DTYPE(dtype, T, { return (launch_forward<T, true>(y, sum, x, residual, w, b, rows, hidden, epsilon, args, s)); });
+    return CGPT_OK;
+}
+
+extern "C" int cgpt_dropout_add_layernorm_backward(void* dx, void* dresidual, void* dw, void* db, const void* dy,
+                                                   const void* dsum, const void* sum, const void* w, void* workspace,
+                                                   size_t workspace_size, size_t rows, size_t hidden, float epsilon,
+                                                   float probability, const uint64_t* state, uint32_t site, int dtype,
+                                                   cgpt_stream_t stream) {
+    if (!dx || !dresidual || !dw || !dy || !sum || !w || !workspace) return CGPT_ERR_NULL;
+    if (!valid_float_dtype(dtype)) return CGPT_ERR_DTYPE;
+    if (!valid_rows(rows, hidden) || workspace_size < workspace_bytes(rows, hidden)) return CGPT_ERR_SHAPE;
+    if (!(epsilon > 0.f) || dx == dresidual || dx == dy || dx == sum || dx == dsum || dresidual == dy || dresidual == sum) return CGPT_ERR_OPTION;
+    if (!element_aligned(dtype, {dx, dresidual, dw, db, dy, dsum, sum, w}) || !aligned16(workspace)) return CGPT_ERR_ALIGN;
+    DropoutArgs args;
+    CGPT_TRY(dropout_args(&args, probability, state, site, rows * hidden));
+    auto s = static_cast<cudaStream_t>(stream);
+    CGPT_DISPATCH_DTYPE(dtype, T, {
+        return (launch_backward<T, true>(dresidual, dx, dw, db, dy, sum, w, dsum, workspace, rows, hidden, epsilon, args, s));
+    });
+    return CGPT_OK;
+}

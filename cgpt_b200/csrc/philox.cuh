@@ -1,0 +1,103 @@
+// Counter-based dropout decisions: Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", SC 2011), one 128-bit block per eight elements.
+//
+// Element e of a tensor (row-major index) takes 16 bits of the block with
+//     key = (seed low, seed high), counter = (e / 8, site, step low, step high):
+// half e % 8 of the four words, low halves first. It is kept where those bits are >= threshold = round(65536 p) and then
+// multiplied by 65536 / (65536 - threshold), so the expectation is exact for the probability that is realised (p in steps of
+// 2^-16). Forward and backward recompute the same bits; no mask is stored. seed and step are read from device memory
+// ({seed, step}, two 64-bit words), so that a captured graph draws new masks when the step is advanced between replays.
+//
+// Sixteen bits a decision, not 32: a block's ten rounds (two 32x32->64 products, four XORs and two key additions each) then
+// cover 16 bytes of a 16-bit tensor, about 8 instructions an element, which stays below what the memory pipe takes.
+#pragma once
+
+#include <cmath>
+#include <initializer_list>
+
+#include "common.cuh"
+
+namespace cgpt {
+
+struct DropoutArgs {
+    const unsigned long long* state;   // {seed, step} in device memory; not read when threshold == 0
+    std::uint32_t site;
+    std::uint32_t threshold;           // 0: nothing is dropped
+    float scale;                       // 65536 / (65536 - threshold)
+};
+
+// The generator of one call with seed, step and site in registers.
+struct Philox {
+    std::uint32_t k0, k1, site, step_lo, step_hi;
+
+    __device__ __forceinline__ explicit Philox(const DropoutArgs& a) {
+        const unsigned long long seed = a.threshold != 0 ? a.state[0] : 0ull, step = a.threshold != 0 ? a.state[1] : 0ull;
+        k0 = static_cast<std::uint32_t>(seed);
+        k1 = static_cast<std::uint32_t>(seed >> 32);
+        step_lo = static_cast<std::uint32_t>(step);
+        step_hi = static_cast<std::uint32_t>(step >> 32);
+        site = a.site;
+    }
+    __device__ __forceinline__ uint4 block(std::uint32_t index) const {
+        uint4 c = make_uint4(index, site, step_lo, step_hi);
+        std::uint32_t ka = k0, kb = k1;
+#pragma unroll
+        for (int r = 0; r < 10; ++r) {
+            const unsigned long long p = static_cast<unsigned long long>(0xD2511F53u) * c.x;
+            const unsigned long long q = static_cast<unsigned long long>(0xCD9E8D57u) * c.z;
+            c = make_uint4(static_cast<std::uint32_t>(q >> 32) ^ c.y ^ ka, static_cast<std::uint32_t>(q),
+                           static_cast<std::uint32_t>(p >> 32) ^ c.w ^ kb, static_cast<std::uint32_t>(p));
+            ka += 0x9E3779B9u;
+            kb += 0xBB67AE85u;
+        }
+        return c;
+    }
+};
+
+// One element's decision on 16 bits. The product is rounded by itself (no contraction with a residual added to it), so that every
+// kernel gives the same bits for the same element.
+__device__ __forceinline__ float decide(float v, std::uint32_t u, std::uint32_t threshold, float scale) {
+    return u >= threshold ? __fmul_rn(v, scale) : 0.f;
+}
+
+// Applies a block's eight decisions to eight consecutive elements. Dropped elements become +0 whatever they held.
+__device__ __forceinline__ void apply_block(float (&v)[8], const uint4& bits, std::uint32_t threshold, float scale) {
+    const std::uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const std::uint32_t u = (i & 1) != 0 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+        v[i] = decide(v[i], u, threshold, scale);
+    }
+}
+
+// The decision of one element, for places that cannot share a block (its other seven decisions are thrown away).
+__device__ __forceinline__ float apply_one(float v, const Philox& gen, long long e, const DropoutArgs& a) {
+    const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
+    const int i = static_cast<int>(e & 7);
+    const std::uint32_t w = i < 4 ? (i < 2 ? c.x : c.y) : (i < 6 ? c.z : c.w);
+    const std::uint32_t u = (i & 1) != 0 ? w >> 16 : w & 0xffffu;
+    return decide(v, u, a.threshold, a.scale);
+}
+
+// Whether every pointer given (NULL ones aside) is aligned to an element of `dtype`.
+inline bool element_aligned(int dtype, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if ((reinterpret_cast<std::uintptr_t>(p) & (dtype_size(dtype) - 1)) != 0) return false;
+    return true;
+}
+
+// Checks the options of a call with dropout over `elements` elements and fills `out`. A probability of 0 reads no state.
+inline int dropout_args(DropoutArgs* out, float probability, const void* state, std::uint32_t site, unsigned long long elements) {
+    *out = DropoutArgs{static_cast<const unsigned long long*>(state), site, 0u, 1.0f};
+    if (!(probability >= 0.f && probability < 1.f)) return CGPT_ERR_OPTION;
+    if (probability == 0.f) return CGPT_OK;
+    if (state == nullptr) return CGPT_ERR_NULL;
+    if ((reinterpret_cast<std::uintptr_t>(state) & 7u) != 0) return CGPT_ERR_ALIGN;
+    if (elements > (1ull << 35)) return CGPT_ERR_SHAPE;   // the block counter has 32 bits
+    const double t = std::nearbyint(static_cast<double>(probability) * 65536.0);
+    out->threshold = static_cast<std::uint32_t>(t > 65535.0 ? 65535.0 : t);
+    out->scale = static_cast<float>(65536.0 / (65536.0 - static_cast<double>(out->threshold)));
+    return CGPT_OK;
+}
+
+}  // namespace cgpt

@@ -6,7 +6,8 @@ of ``std::invalid_argument``. Tensors are ``torch`` CUDA tensors used purely as 
 all arithmetic happens in ``libcgpt_b200.so`` through the C ABI.
 
 Reference declarations: ``include/ops/backward/*.h``, ``include/ops/{rmsnorm,rope,swiglu,embedding,
-cross_entropy,cut_cross_entropy}.h``.
+cross_entropy,cut_cross_entropy}.h``. The operators of the pre-norm block (dropout, layer norm, the two fused with the residual
+add, scaled embedding) have no counterpart there and follow the same conventions.
 """
 from __future__ import annotations
 
@@ -416,6 +417,223 @@ def add_tensors(output, a, b, stream=None, c=None):
     _require(output.shape == a.shape == b.shape, "add_tensors: shapes differ")
     check(lib.cgpt_add(ptr(output), ptr(a), ptr(b), ptr(c), a.numel(), dtype_code(a), stream_ptr(stream)),
           "add_tensors")
+
+
+# ----------------------------------------------------------- Dropout, layer norm, scaled embedding (pre-norm block)
+@dataclass
+class DropoutOptions:
+    """``probability`` of dropping an element, realised in steps of 2^-16; 0 switches dropout off (the state may then be None).
+    ``site`` tells the dropouts of one step apart: give every call of a step that must draw its own mask another number, and a
+    backward call the number of its forward call."""
+    probability: float = 0.0
+    site: int = 0
+
+
+@dataclass
+class ScaledEmbeddingOptions:
+    """``scale`` multiplies every looked-up row (sqrt(hidden) in many models); tokens whose id is ``padding_id`` take no part in
+    the gradient; ``accumulate_weight`` adds to the gradient table instead of overwriting it."""
+    scale: float = 1.0
+    padding_id: int | None = None
+    dropout: DropoutOptions | None = None
+    accumulate_weight: bool = False
+
+
+_NO_DROPOUT = DropoutOptions()
+
+
+def make_dropout_state(seed: int, step: int = 0, device=None) -> torch.Tensor:
+    """The generator state that the dropout calls of a model share: {seed, step}, two 64-bit words on the device."""
+    signed = lambda v: (v & 0xffffffffffffffff) - ((v & 0x8000000000000000) << 1)
+    return torch.tensor([signed(seed), signed(step)], dtype=torch.int64, device="cuda" if device is None else device)
+
+
+def dropout_advance(state, steps: int = 1, stream=None):
+    """step += steps on the device, after a training step's backward (capturable: replays of a graph that holds this call draw new
+    masks every time)."""
+    _require(steps >= 0, "dropout_advance: steps must not be negative")
+    device = _state_check("dropout_advance", state)
+    check(lib.cgpt_dropout_advance(state.data_ptr(), steps, _stream_on("dropout_advance", device, stream)), "dropout_advance")
+
+
+def _state_check(name, state, device=None):
+    _require(state is not None and state.is_cuda and state.dtype in (torch.int64, torch.uint64) and state.numel() == 2 and state.is_contiguous()
+             and (device is None or state.get_device() == device), f"{name}: state must be two 64-bit words on the tensors' device")
+    return state.get_device()
+
+
+def _dropout_options(name, options, state, device):
+    """(probability, state pointer, site) of a call."""
+    o = options or _NO_DROPOUT
+    _require(0.0 <= o.probability < 1.0, f"{name}: probability must be in [0, 1)")
+    _require(0 <= o.site <= 0xffffffff, f"{name}: site must fit 32 bits")
+    if o.probability == 0.0:
+        return 0.0, None, o.site
+    _state_check(name, state, device)
+    return o.probability, state.data_ptr(), o.site
+
+
+def _stream_on(name, device, stream):
+    """Stream pointer of a call whose tensors are on `device`, which has to be the current device and the stream's."""
+    _require(device == torch.cuda.current_device() and (stream is None or stream.device_index == device),
+             f"{name}: tensors and stream must be on the current device")
+    return stream_ptr(stream)
+
+
+def _one_device(name, *tensors):
+    """Device index of contiguous CUDA tensors of one dtype (None is skipped)."""
+    first = tensors[0]
+    device, dtype = first.get_device(), first.dtype
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.dtype == dtype and t.get_device() == device and t.is_contiguous()):
+            _same_cuda_dtype(name, *[u for u in tensors if u is not None])
+            _require(False, f"{name}: all tensors must be on one device")
+    return device
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(name, workspace, size, device, stream):
+    """The caller's workspace, or one allocated on the call's stream. (pointer, bytes, the tensor to keep alive)"""
+    if workspace is None:
+        if stream is None:
+            workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        else:
+            with torch.cuda.stream(stream):   # its memory is handed on in this stream's order
+                workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        return workspace.data_ptr(), size, workspace
+    have = workspace.numel() * workspace.element_size()
+    _require(workspace.is_cuda and workspace.get_device() == device and workspace.is_contiguous() and have >= size,
+             f"{name}: workspace must be a contiguous CUDA buffer of at least {size} bytes on the tensors' device")
+    return workspace.data_ptr(), have, workspace
+
+
+def dropout_forward(output, input, state, stream=None, options: DropoutOptions | None = None, residual=None):
+    """output = [residual +] dropout(input), any shape. output may be input or residual itself."""
+    device = _one_device("dropout_forward", output, input, residual)
+    _require(output.shape == input.shape and (residual is None or residual.shape == input.shape), "dropout_forward: shapes differ")
+    p, state_ptr, site = _dropout_options("dropout_forward", options, state, device)
+    check(lib.cgpt_dropout_forward(output.data_ptr(), input.data_ptr(), _ptr(residual), input.numel(), p, state_ptr, site,
+                                   dtype_code(input), _stream_on("dropout_forward", device, stream)), "dropout_forward")
+
+
+def dropout_backward(grad_input, grad_output, state, stream=None, options: DropoutOptions | None = None,
+                     accumulate_input: bool = False):
+    """grad_input = [grad_input +] the dropout map of grad_output; the forward's state, unadvanced, and its options."""
+    device = _one_device("dropout_backward", grad_input, grad_output)
+    _require(grad_input.shape == grad_output.shape, "dropout_backward: shapes differ")
+    p, state_ptr, site = _dropout_options("dropout_backward", options, state, device)
+    check(lib.cgpt_dropout_backward(grad_input.data_ptr(), grad_output.data_ptr(), grad_output.numel(), p, state_ptr, site,
+                                    int(accumulate_input), dtype_code(grad_output), _stream_on("dropout_backward", device, stream)),
+          "dropout_backward")
+
+
+def _norm_shapes(name, x, weight, rows_like, vectors):
+    _require(x.dim() == 2 and weight.dim() == 1 and weight.shape[0] == x.shape[1], f"{name}: incompatible shapes")
+    for t in rows_like:
+        _require(t is None or t.shape == x.shape, f"{name}: incompatible shapes")
+    for t in vectors:
+        _require(t is None or t.shape == weight.shape, f"{name}: incompatible shapes")
+
+
+def layernorm_forward(output, input, weight, bias, epsilon, stream=None):
+    """output = (input - mean) / sqrt(var + epsilon) * weight + bias over rows of a matrix; bias may be None."""
+    device = _one_device("layernorm_forward", output, input, weight, bias)
+    _norm_shapes("layernorm_forward", input, weight, (output,), (bias,))
+    check(lib.cgpt_layernorm_forward(output.data_ptr(), input.data_ptr(), weight.data_ptr(), _ptr(bias), input.shape[0], input.shape[1],
+                                     epsilon, dtype_code(input), _stream_on("layernorm_forward", device, stream)), "layernorm_forward")
+
+
+def layernorm_backward(grad_input, grad_weight, grad_bias, grad_output, input, weight, epsilon, stream=None, residual=None,
+                       workspace=None):
+    """Gradients of layernorm_forward (statistics are recomputed from input). grad_bias may be None; ``residual`` is added to
+    grad_input inside the kernel. ``workspace``: a buffer of layernorm_backward_workspace_bytes(rows, hidden) bytes, allocated
+    on the call's stream when None."""
+    device = _one_device("layernorm_backward", grad_input, grad_weight, grad_bias, grad_output, input, weight, residual)
+    _norm_shapes("layernorm_backward", input, weight, (grad_input, grad_output, residual), (grad_weight, grad_bias))
+    rows, hidden = input.shape
+    s = _stream_on("layernorm_backward", device, stream)
+    at, size, keep = _workspace("layernorm_backward", workspace, layernorm_backward_workspace_bytes(rows, hidden), device, stream)
+    check(lib.cgpt_layernorm_backward(grad_input.data_ptr(), grad_weight.data_ptr(), _ptr(grad_bias), grad_output.data_ptr(),
+                                      input.data_ptr(), weight.data_ptr(), _ptr(residual), at, size, rows, hidden, epsilon,
+                                      dtype_code(input), s), "layernorm_backward")
+
+
+def layernorm_backward_workspace_bytes(rows: int, hidden: int) -> int:
+    """Workspace of layernorm_backward and dropout_add_layernorm_backward."""
+    return lib.cgpt_layernorm_backward_workspace_bytes(rows, hidden)
+
+
+def dropout_add_layernorm_forward(output, sum, input, residual, weight, bias, epsilon, state, stream=None,
+                                  options: DropoutOptions | None = None):
+    """sum = residual + dropout(input); output = layernorm(sum), in one pass. sum may be input or residual itself."""
+    name = "dropout_add_layernorm_forward"
+    device = _one_device(name, output, sum, input, residual, weight, bias)
+    _norm_shapes(name, input, weight, (output, sum, residual), (bias,))
+    p, state_ptr, site = _dropout_options(name, options, state, device)
+    check(lib.cgpt_dropout_add_layernorm_forward(output.data_ptr(), sum.data_ptr(), input.data_ptr(), residual.data_ptr(),
+                                                 weight.data_ptr(), _ptr(bias), input.shape[0], input.shape[1], epsilon, p, state_ptr,
+                                                 site, dtype_code(input), _stream_on(name, device, stream)), name)
+
+
+def dropout_add_layernorm_backward(grad_input, grad_residual, grad_weight, grad_bias, grad_output, grad_sum, sum, weight, epsilon,
+                                   state, stream=None, options: DropoutOptions | None = None, workspace=None):
+    """Gradients of dropout_add_layernorm_forward from those of its output and (None: zero) of its sum. grad_residual may be
+    grad_sum itself; grad_bias may be None. ``workspace`` as in layernorm_backward."""
+    name = "dropout_add_layernorm_backward"
+    device = _one_device(name, grad_input, grad_residual, grad_weight, grad_bias, grad_output, grad_sum, sum, weight)
+    _norm_shapes(name, sum, weight, (grad_input, grad_residual, grad_output, grad_sum), (grad_weight, grad_bias))
+    rows, hidden = sum.shape
+    p, state_ptr, site = _dropout_options(name, options, state, device)
+    s = _stream_on(name, device, stream)
+    at, size, keep = _workspace(name, workspace, layernorm_backward_workspace_bytes(rows, hidden), device, stream)
+    check(lib.cgpt_dropout_add_layernorm_backward(grad_input.data_ptr(), grad_residual.data_ptr(), grad_weight.data_ptr(), _ptr(grad_bias),
+                                                  grad_output.data_ptr(), _ptr(grad_sum), sum.data_ptr(), weight.data_ptr(), at, size,
+                                                  rows, hidden, epsilon, p, state_ptr, site, dtype_code(sum), s), name)
+
+
+_NO_EMBEDDING_OPTIONS = ScaledEmbeddingOptions()
+
+
+def _embedding_check(name, table, activations, ids, token_count, options, state):
+    device = _one_device(name, table, activations)
+    _ids(ids, token_count, name)
+    _require(ids.get_device() == device and ids.is_contiguous(), f"{name}: token ids must be contiguous and on the tensors' device")
+    _require(table.dim() == 2 and token_count > 0 and activations.numel() == token_count * table.shape[1],
+             f"{name}: activations must hold token_count * hidden elements")
+    return device, _dropout_options(name, options.dropout, state, device)
+
+
+def scaled_embedding_forward(output, device_token_ids, token_count, weight, state=None, stream=None,
+                             options: ScaledEmbeddingOptions | None = None):
+    """output[t] = dropout(scale * weight[ids[t]]); ids outside the table give zero rows."""
+    o = options or _NO_EMBEDDING_OPTIONS
+    device, (p, state_ptr, site) = _embedding_check("scaled_embedding_forward", weight, output, device_token_ids, token_count, o, state)
+    check(lib.cgpt_scaled_embedding_forward(output.data_ptr(), device_token_ids.data_ptr(), weight.data_ptr(), token_count, weight.shape[0],
+                                            weight.shape[1], o.scale, p, state_ptr, site, dtype_code(weight),
+                                            _stream_on("scaled_embedding_forward", device, stream)), "scaled_embedding_forward")
+
+
+def scaled_embedding_backward(grad_weight, grad_output, device_token_ids, token_count, state=None, stream=None,
+                              options: ScaledEmbeddingOptions | None = None, workspace=None):
+    """grad_weight[v] (+)= scale * the sum of the dropout map of grad_output over the tokens with id v. ``workspace``: a buffer of
+    scaled_embedding_backward_workspace_bytes(token_count, hidden) bytes, allocated on the call's stream when None."""
+    name = "scaled_embedding_backward"
+    o = options or _NO_EMBEDDING_OPTIONS
+    device, (p, state_ptr, site) = _embedding_check(name, grad_weight, grad_output, device_token_ids, token_count, o, state)
+    _require(o.padding_id is None or 0 <= o.padding_id < grad_weight.shape[0], f"{name}: padding_id must be a row of the table")
+    vocab, hidden = grad_weight.shape
+    s = _stream_on(name, device, stream)
+    at, size, keep = _workspace(name, workspace, scaled_embedding_backward_workspace_bytes(token_count, hidden), device, stream)
+    check(lib.cgpt_scaled_embedding_backward(grad_weight.data_ptr(), grad_output.data_ptr(), device_token_ids.data_ptr(), at, size,
+                                             token_count, vocab, hidden, o.scale, 0xffffffff if o.padding_id is None else o.padding_id,
+                                             p, state_ptr, site, int(o.accumulate_weight), dtype_code(grad_weight), s), name)
+
+
+def scaled_embedding_backward_workspace_bytes(token_count: int, hidden: int) -> int:
+    return lib.cgpt_scaled_embedding_backward_workspace_bytes(token_count, hidden)
 
 
 # --------------------------------------------------------------------------------------- Cross entropy

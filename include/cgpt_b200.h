@@ -289,6 +289,68 @@ int cgpt_add(void* out, const void* a, const void* b, const void* c, size_t coun
              cgpt_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Operators of the pre-norm block that the reference does not have: dropout, layer norm, the two fused with the residual
+ * add, and an embedding with scale and dropout. Their kernels take global scratch from the caller (`workspace`,
+ * `workspace_size` bytes, 16-byte aligned; each *_workspace_bytes gives the size, 0 for invalid sizes), so calls on different
+ * streams and captured graphs share nothing inside the library. The workspace needs no initial value and holds nothing
+ * between calls. Tensors must not overlap unless a parameter says so.
+ *
+ * Dropout. Element e (row-major index) of a call's tensor is decided by 16 bits of Philox4x32-10 with key = seed and counter =
+ * (e / 8, site, step low word, step high word): half e % 8 of the block's four words, low halves first. It is kept where those
+ * bits are >= t = round(65536 * probability) (at most 65535) and multiplied by 65536 / (65536 - t); dropped elements are 0
+ * whatever they held. `state` is a DEVICE buffer of two 64-bit words {seed, step}; `site` tells the dropouts of one step
+ * apart. Backward calls recompute the mask from the same state, so the step may only advance after them. Since the state is
+ * read on the device, a captured graph draws new masks after cgpt_dropout_advance (itself capturable: step += steps).
+ * 0 <= probability < 1; probability 0 is the identity and does not read `state`, which may then be NULL. At most 2^35 elements.
+ *   forward   out = [residual +] drop(in)      out may be the same buffer as in or residual
+ *   backward  din = [din +] drop(dout)         din may be the same buffer as dout unless accumulate != 0
+ * ---------------------------------------------------------------------------------------------- */
+int cgpt_dropout_forward(void* out, const void* in, const void* residual, size_t count, float probability,
+                         const uint64_t* state, uint32_t site, int dtype, cgpt_stream_t stream);
+int cgpt_dropout_backward(void* din, const void* dout, size_t count, float probability, const uint64_t* state, uint32_t site,
+                          int accumulate, int dtype, cgpt_stream_t stream);
+int cgpt_dropout_advance(uint64_t* state, uint64_t steps, cgpt_stream_t stream);
+
+/* Layer norm  y = (x - mean) rstd w + b,  rstd = 1 / sqrt(var + eps), var = mean((x - mean)^2); x, y, dy, dx: [rows, hidden];
+ * w, b, dw, db: [hidden]. b may be NULL (no bias), db may be NULL (not wanted). fp32 math, one rounding on store.
+ * Backward recomputes mean and rstd from x and overwrites dx, dw, db:  xh = (x - mean) rstd, g = dy w;
+ *      dx = rstd (g - mean(g) - xh mean(g xh)) (+ residual);  dw = sum_rows dy xh;  db = sum_rows dy.
+ * residual may be NULL and may be the same buffer as dx. y may not alias x; dx may alias neither dy nor x. */
+int cgpt_layernorm_forward(void* y, const void* x, const void* w, const void* b, size_t rows, size_t hidden, float epsilon,
+                           int dtype, cgpt_stream_t stream);
+size_t cgpt_layernorm_backward_workspace_bytes(size_t rows, size_t hidden);
+int cgpt_layernorm_backward(void* dx, void* dw, void* db, const void* dy, const void* x, const void* w, const void* residual,
+                            void* workspace, size_t workspace_size, size_t rows, size_t hidden, float epsilon, int dtype,
+                            cgpt_stream_t stream);
+
+/* Sub-layer boundary of a pre-norm block in one pass:  sum = residual + drop(x), y = layernorm(sum), both written; the norm is
+ * of the rounded sum, so results equal cgpt_dropout_forward followed by cgpt_layernorm_forward. sum may be the same buffer as
+ * x or residual. Backward takes the gradient of y and (unless NULL) that of sum from the residual path:
+ *      dresidual = dsum + layernorm_backward(dy; sum, w),  dx = drop(dresidual before its rounding),  dw, db.
+ * dresidual may be the same buffer as dsum. Workspace: cgpt_layernorm_backward_workspace_bytes(rows, hidden). */
+int cgpt_dropout_add_layernorm_forward(void* y, void* sum, const void* x, const void* residual, const void* w, const void* b,
+                                       size_t rows, size_t hidden, float epsilon, float probability, const uint64_t* state,
+                                       uint32_t site, int dtype, cgpt_stream_t stream);
+int cgpt_dropout_add_layernorm_backward(void* dx, void* dresidual, void* dw, void* db, const void* dy, const void* dsum,
+                                        const void* sum, const void* w, void* workspace, size_t workspace_size, size_t rows,
+                                        size_t hidden, float epsilon, float probability, const uint64_t* state, uint32_t site,
+                                        int dtype, cgpt_stream_t stream);
+
+/* Embedding with a scale and dropout:  out[t, :] = drop(scale * weight[ids[t], :]); an id outside the table gives a zero row.
+ * Backward: grad_weight[v, :] (+)= scale * sum over tokens t with ids[t] = v of drop(grad_output[t, :]), summed in fp32 in an
+ * order that follows from the ids alone and rounded once; tokens whose id is padding_id (UINT32_MAX: none) or outside the table
+ * are skipped. accumulate == 0 writes every row of the table (zeros where no token points), else rows without tokens stay as
+ * they are. tokens < 2^31. ids: uint32. */
+int cgpt_scaled_embedding_forward(void* out, const uint32_t* ids, const void* weight, size_t tokens, size_t vocab, size_t hidden,
+                                  float scale, float probability, const uint64_t* state, uint32_t site, int dtype,
+                                  cgpt_stream_t stream);
+size_t cgpt_scaled_embedding_backward_workspace_bytes(size_t tokens, size_t hidden);
+int cgpt_scaled_embedding_backward(void* grad_weight, const void* grad_output, const uint32_t* ids, void* workspace,
+                                   size_t workspace_size, size_t tokens, size_t vocab, size_t hidden, float scale,
+                                   uint32_t padding_id, float probability, const uint64_t* state, uint32_t site, int accumulate,
+                                   int dtype, cgpt_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Softmax cross-entropy on materialised logits.
  * Replaces cross_entropy_forward_backward / cross_entropy_forward (reference
  * include/ops/cross_entropy.h:25-42, src/ops/cross_entropy.cu:352-410).
