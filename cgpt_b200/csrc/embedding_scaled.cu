@@ -27,25 +27,6 @@ constexpr int kSortTile = kSortThreads * kKeysPerThread;
 constexpr int kMaxDigitBits = 9;
 constexpr int kChunk = 32;           // sorted tokens per chunk
 
-// The dropout map of VEC elements that start at element e of the tensor (e % VEC == 0 for VEC > 1).
-template <int VEC>
-__device__ __forceinline__ void drop_vec(float (&v)[VEC], const Philox& gen, long long e, const DropoutArgs& args) {
-    if constexpr (VEC == 8) {
-        apply_block(v, gen.block(static_cast<std::uint32_t>(e >> 3)), args.threshold, args.scale);
-    } else if constexpr (VEC == 4) {
-        const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
-        const bool high = (e & 4) != 0;
-        const std::uint32_t w0 = high ? c.z : c.x, w1 = high ? c.w : c.y;
-        v[0] = decide(v[0], w0 & 0xffffu, args.threshold, args.scale);
-        v[1] = decide(v[1], w0 >> 16, args.threshold, args.scale);
-        v[2] = decide(v[2], w1 & 0xffffu, args.threshold, args.scale);
-        v[3] = decide(v[3], w1 >> 16, args.threshold, args.scale);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = apply_one(v[i], gen, e + i, args);
-    }
-}
-
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
 scaled_embedding_forward_kernel(T* __restrict__ out, const std::uint32_t* __restrict__ ids, const T* __restrict__ weight,

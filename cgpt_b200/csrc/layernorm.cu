@@ -12,6 +12,8 @@
 // (per-CTA partial rows, then one pass over them), so results repeat bit for bit.
 //
 // Memory-bound: 2 * H * sizeof(T) bytes per row forward, 3 backward (+1 with a residual), 4 and 5 for the fused pair.
+#include <type_traits>
+
 #include "philox.cuh"
 #include "launch_counter.h"
 
@@ -176,6 +178,49 @@ layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __r
     }
 }
 
+template <int N>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i] = v[i];
+    }
+}
+
+#include "layernorm_rows.cuh"
+
+// How a call's rows are laid out: threads per row, row groups per CTA and CTAs. vec == 0: the kernels for rows of any length.
+struct Plan {
+    int vec, cpt, tpr, groups;
+    unsigned grid;
+};
+
+// CTAs per SM a rows kernel may have: 512 threads of at most 128 registers.
+constexpr int kResidentThreads = 512;
+
+// vector: all tensors 16-byte aligned. The layout depends on the sizes and the alignment alone, not on which operator is called,
+// so that the fused operators give the bits of their parts.
+Plan make_plan(std::size_t rows, std::size_t hidden, std::size_t elem, bool vector) {
+    const int full = static_cast<int>(16 / elem);
+    Plan p{};
+    p.vec = vector && hidden % full == 0 ? full : 1;
+    const std::size_t vectors = hidden / p.vec;
+    const int options[3] = {p.vec > 1 ? 1 : 4, p.vec > 1 ? 2 : 16, p.vec > 1 ? 4 : 16};
+    int i = 0;
+    while (i < 2 && vectors > static_cast<std::size_t>(rows_kernels::kMaxTpr) * options[i]) ++i;
+    p.cpt = options[i];
+    if (vectors > static_cast<std::size_t>(rows_kernels::kMaxTpr) * p.cpt) return Plan{};
+    const int rows_at_once = p.vec > 1 ? 4 / p.cpt : (p.cpt == 4 ? 2 : 1);
+    p.tpr = static_cast<int>((vectors + p.cpt * 32 - 1) / (p.cpt * 32)) * 32;
+    p.groups = p.tpr < 256 ? 256 / p.tpr : 1;
+    const std::size_t need = (rows + p.groups * rows_at_once - 1) / (p.groups * rows_at_once);
+    const std::size_t cap = static_cast<std::size_t>(kNumSMs) * (kResidentThreads / (p.groups * p.tpr));
+    p.grid = static_cast<unsigned>(need < cap ? need : cap);
+    return p;
+}
+
 constexpr std::size_t kMaxSplits = 64;
 std::size_t any_splits(std::size_t rows) {
     const std::size_t n = (rows + 63) / 64;
@@ -188,13 +233,48 @@ bool valid_rows(std::size_t rows, std::size_t hidden) {
     return rows != 0 && hidden != 0 && hidden <= 0x7fffffffull && rows <= (1ull << 46) / hidden;
 }
 
+// Enough for the call's layout whatever its type and alignment turn out to be.
 std::size_t workspace_bytes(std::size_t rows, std::size_t hidden) {
-    return rows * sizeof(float2) + any_splits(rows) * 2 * hidden * sizeof(float);
+    std::size_t parts = 0, stats = 0;
+    for (std::size_t elem : {2, 4})
+        for (bool vector : {false, true}) {
+            const Plan p = make_plan(rows, hidden, elem, vector);
+            const std::size_t n = p.vec != 0 ? p.grid : any_splits(rows);
+            if (n > parts) parts = n;
+            if (p.vec == 0) stats = rows * sizeof(float2);
+        }
+    return parts * 2 * hidden * sizeof(float) + stats;
+}
+
+// Calls `f` with the plan's vector width, vectors per thread and rows at a time as compile-time constants.
+template <typename T, typename F>
+int with_layout(const Plan& p, F f) {
+    constexpr int V = 16 / sizeof(T);
+#define CGPT_LAYOUT(VEC, CPT, R) f(std::integral_constant<int, VEC>{}, std::integral_constant<int, CPT>{}, std::integral_constant<int, R>{})
+    if (p.vec == V) return p.cpt == 1 ? CGPT_LAYOUT(V, 1, 4) : p.cpt == 2 ? CGPT_LAYOUT(V, 2, 2) : CGPT_LAYOUT(V, 4, 1);
+    return p.cpt == 4 ? CGPT_LAYOUT(1, 4, 2) : CGPT_LAYOUT(1, 16, 1);
+#undef CGPT_LAYOUT
 }
 
 template <typename T, bool FUSED>
 int launch_forward(void* y, void* sum, const void* x, const void* residual, const void* w, const void* b, std::size_t rows,
                    std::size_t hidden, float epsilon, const DropoutArgs& args, cudaStream_t s) {
+    const bool al = aligned16(y) && aligned16(sum) && aligned16(x) && aligned16(residual) && aligned16(w) && aligned16(b);
+    const Plan p = make_plan(rows, hidden, sizeof(T), al);
+    if (p.vec != 0)
+        return with_layout<T>(p, [&](auto vec, auto cpt, auto r) {
+            auto kernel = rows_kernels::layernorm_forward_rows_kernel<T, vec.value, cpt.value, r.value, FUSED>;
+            const int threads = p.groups * p.tpr;
+            const std::size_t at_once = static_cast<std::size_t>(p.groups) * r.value, need = (rows + at_once - 1) / at_once;
+            const std::size_t cap = static_cast<std::size_t>(kNumSMs) * resident_ctas_per_sm(reinterpret_cast<const void*>(kernel), threads, 0);
+            kernel<<<static_cast<unsigned>(need < cap ? need : cap), threads, 0, s>>>(
+                static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
+                static_cast<const T*>(w), static_cast<const T*>(b), static_cast<long long>(rows), static_cast<int>(hidden), epsilon,
+                p.tpr, args);
+            count_launch();
+            CGPT_LAUNCH_CHECK();
+            return CGPT_OK;
+        });
     layernorm_forward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
         static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
         static_cast<const T*>(w), static_cast<const T*>(b), static_cast<long long>(rows), static_cast<long long>(hidden), epsilon, args);
@@ -206,8 +286,31 @@ int launch_forward(void* y, void* sum, const void* x, const void* residual, cons
 template <typename T, bool FUSED>
 int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, const void* x, const void* w, const void* residual,
                     void* workspace, std::size_t rows, std::size_t hidden, float epsilon, const DropoutArgs& args, cudaStream_t s) {
-    const std::size_t splits = any_splits(rows);
     float* partial = static_cast<float*>(workspace);
+    const unsigned columns = static_cast<unsigned>((hidden + 31) / 32);
+    auto reduce = [&](std::size_t parts) {
+        layernorm_reduce_kernel<T><<<dim3(columns, db != nullptr ? 2 : 1), 1024, 0, s>>>(
+            static_cast<T*>(dw), static_cast<T*>(db), partial, static_cast<int>(parts), static_cast<long long>(hidden));
+        count_launch();
+        CGPT_LAUNCH_CHECK();
+        return CGPT_OK;
+    };
+    const bool al = aligned16(dx) && aligned16(din) && aligned16(dy) && aligned16(x) && aligned16(w) && aligned16(residual);
+    const Plan p = make_plan(rows, hidden, sizeof(T), al);
+    if (p.vec != 0)
+        return with_layout<T>(p, [&](auto vec, auto cpt, auto r) {
+            const std::size_t sums = static_cast<std::size_t>(p.groups) * 4 * r.value * 16 * sizeof(float);
+            const std::size_t parts = p.groups > 1 ? static_cast<std::size_t>(2) * cpt.value * vec.value * p.tpr * sizeof(float) : 0;
+            rows_kernels::layernorm_backward_rows_kernel<T, vec.value, cpt.value, r.value, FUSED>
+                <<<p.grid, p.groups * p.tpr, sums > parts ? sums : parts, s>>>(
+                    static_cast<T*>(dx), static_cast<T*>(din), partial, static_cast<const T*>(dy), static_cast<const T*>(x),
+                    static_cast<const T*>(w), static_cast<const T*>(residual), static_cast<long long>(rows), static_cast<int>(hidden),
+                    epsilon, p.tpr, args);
+            count_launch();
+            CGPT_LAUNCH_CHECK();
+            return reduce(p.grid);
+        });
+    const std::size_t splits = any_splits(rows);
     float2* stats = reinterpret_cast<float2*>(partial + splits * 2 * hidden);
     layernorm_backward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
         static_cast<T*>(dx), static_cast<T*>(din), stats, static_cast<const T*>(dy), static_cast<const T*>(x),
@@ -215,16 +318,11 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
         epsilon, args);
     count_launch();
     CGPT_LAUNCH_CHECK();
-    const unsigned columns = static_cast<unsigned>((hidden + 31) / 32);
     layernorm_columns_any_kernel<T><<<dim3(columns, static_cast<unsigned>(splits)), kThreads, 0, s>>>(
         partial, static_cast<const T*>(dy), static_cast<const T*>(x), stats, static_cast<long long>(rows), static_cast<long long>(hidden));
     count_launch();
     CGPT_LAUNCH_CHECK();
-    layernorm_reduce_kernel<T><<<dim3(columns, db != nullptr ? 2 : 1), 1024, 0, s>>>(
-        static_cast<T*>(dw), static_cast<T*>(db), partial, static_cast<int>(splits), static_cast<long long>(hidden));
-    count_launch();
-    CGPT_LAUNCH_CHECK();
-    return CGPT_OK;
+    return reduce(splits);
 }
 
 }  // namespace
