@@ -16,8 +16,12 @@
 
 #include "philox.cuh"
 #include "launch_counter.h"
+#include "sm100.cuh"
 
 namespace cgpt {
+
+unsigned int* tc_status_device_ptr();   // gemm.cu: status word raised when a bounded device-side wait runs out
+
 namespace {
 
 constexpr int kThreads = 256;
@@ -55,6 +59,65 @@ __device__ __forceinline__ void norm_sums(float (&s)[3], float dy, float w, floa
     s[1] = fmaf(dy, w, s[1]);
     s[2] = fmaf(__fmul_rn(dy, w), d, s[2]);
 }
+
+// Sums NV values over a warp. Halves the set of values a lane is responsible for while lanes still differ in what they hold, so
+// NV = 4 takes 6 shuffles and NV = 12 takes 18 (5 NV one value at a time). Afterwards lane l holds, in v[0 .. count), the
+// totals of the values first_of(l) .. first_of(l) + count.
+template <int NV>
+struct WarpSums {
+    static constexpr int kFirst = NV % 2 == 0 ? NV / 2 : NV;
+    static constexpr int kCount = NV % 4 == 0 ? NV / 4 : kFirst;
+    static __device__ __forceinline__ int first_of(int lane) {
+        int f = 0;
+        if constexpr (NV % 2 == 0) f += ((lane >> 4) & 1) * (NV / 2);
+        if constexpr (NV % 4 == 0) f += ((lane >> 3) & 1) * (NV / 4);
+        return f;
+    }
+    // A lane of those that hold value i.
+    static __device__ __forceinline__ constexpr int holder_of(int i) {
+        int l = 0;
+        if (NV % 2 == 0 && i >= NV / 2) { l += 16; i -= NV / 2; }
+        if (NV % 4 == 0 && i >= NV / 4) l += 8;
+        return l;
+    }
+    static __device__ __forceinline__ void reduce(float (&v)[NV], int lane) {
+        if constexpr (NV % 2 == 0) {
+            const bool up = (lane & 16) != 0;
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) {
+                const float send = up ? v[i] : v[i + NV / 2], keep = up ? v[i + NV / 2] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 16);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+        }
+        if constexpr (NV % 4 == 0) {
+            const bool up = (lane & 8) != 0;
+#pragma unroll
+            for (int i = 0; i < NV / 4; ++i) {
+                const float send = up ? v[i] : v[i + NV / 4], keep = up ? v[i + NV / 4] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 8);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kFirst; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 8);
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        }
+    }
+    // Every lane gets every total.
+    static __device__ __forceinline__ void broadcast(float (&v)[NV]) {
+        float t[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) t[i] = __shfl_sync(0xffffffffu, v[i % kCount], holder_of(i));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = t[i];
+    }
+};
 
 // ------------------------------------------------------------------------------------------ rows of any length
 // One CTA per row, the row read again (from L1/L2) for every pass over it. Any H, any alignment.
@@ -178,45 +241,101 @@ layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __r
     }
 }
 
-template <int N>
-__device__ __forceinline__ void store_floats(float* p, const float (&v)[N]) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = v[i];
-    }
+#include "layernorm_rows.cuh"
+#include "layernorm_ring.cuh"
+
+// How a call's rows are laid out. It follows from the sizes and the alignment alone, not from which operator is called, so that
+// the fused operators give the bits of their parts.
+enum class Form { kAny, kRows, kRing };
+
+constexpr std::size_t kSmemPerSm = 222 * 1024;   // what the resident CTAs of an SM share, less what the hardware keeps
+
+// Rings take rows of which shared memory holds two stages of both tensors of the fused forward beside w and b (14016 16-bit
+// or 8192 fp32 elements).
+Form form_of(std::size_t hidden, std::size_t elem, bool vector) {
+    if (vector && hidden * elem % 16 == 0)
+        return hidden * elem / 16 <= 2048 && ring_kernels::kVectorsOffset + 2 * hidden * sizeof(float) + 4 * hidden * elem <= kSmemPerSm ? Form::kRing : Form::kAny;
+    return hidden <= 16 * rows_kernels::kMaxTpr ? Form::kRows : Form::kAny;
 }
 
-#include "layernorm_rows.cuh"
-
-// How a call's rows are laid out: threads per row, row groups per CTA and CTAs. vec == 0: the kernels for rows of any length.
-struct Plan {
-    int vec, cpt, tpr, groups;
+// Rows of single elements: threads per row, row groups per CTA and (backward, 512 threads of up to 128 registers per SM) CTAs.
+struct RowsPlan {
+    int cpt, tpr, groups;
     unsigned grid;
 };
-
-// CTAs per SM a rows kernel may have: 512 threads of at most 128 registers.
-constexpr int kResidentThreads = 512;
-
-// vector: all tensors 16-byte aligned. The layout depends on the sizes and the alignment alone, not on which operator is called,
-// so that the fused operators give the bits of their parts.
-Plan make_plan(std::size_t rows, std::size_t hidden, std::size_t elem, bool vector) {
-    const int full = static_cast<int>(16 / elem);
-    Plan p{};
-    p.vec = vector && hidden % full == 0 ? full : 1;
-    const std::size_t vectors = hidden / p.vec;
-    const int options[3] = {p.vec > 1 ? 1 : 4, p.vec > 1 ? 2 : 16, p.vec > 1 ? 4 : 16};
-    int i = 0;
-    while (i < 2 && vectors > static_cast<std::size_t>(rows_kernels::kMaxTpr) * options[i]) ++i;
-    p.cpt = options[i];
-    if (vectors > static_cast<std::size_t>(rows_kernels::kMaxTpr) * p.cpt) return Plan{};
-    const int rows_at_once = p.vec > 1 ? 4 / p.cpt : (p.cpt == 4 ? 2 : 1);
-    p.tpr = static_cast<int>((vectors + p.cpt * 32 - 1) / (p.cpt * 32)) * 32;
+RowsPlan plan_rows(std::size_t rows, std::size_t hidden) {
+    RowsPlan p;
+    p.cpt = hidden <= 4 * rows_kernels::kMaxTpr ? 4 : 16;
+    p.tpr = static_cast<int>((hidden + p.cpt * 32 - 1) / (p.cpt * 32)) * 32;
     p.groups = p.tpr < 256 ? 256 / p.tpr : 1;
-    const std::size_t need = (rows + p.groups * rows_at_once - 1) / (p.groups * rows_at_once);
-    const std::size_t cap = static_cast<std::size_t>(kNumSMs) * (kResidentThreads / (p.groups * p.tpr));
+    const std::size_t at_once = static_cast<std::size_t>(p.groups) * (p.cpt == 4 ? 2 : 1), need = (rows + at_once - 1) / at_once;
+    const std::size_t cap = static_cast<std::size_t>(kNumSMs) * (512 / (p.groups * p.tpr));
+    p.grid = static_cast<unsigned>(need < cap ? need : cap);
+    return p;
+}
+
+struct RingPlan {
+    ring_kernels::RingArgs args;
+    int cpt, cols, threads;
+    unsigned grid;
+    std::size_t smem;
+};
+
+RingPlan plan_ring_common(std::size_t hidden, std::size_t elem) {
+    RingPlan p{};
+    const int v = static_cast<int>(hidden * elem / 16);
+    p.args.vectors = v;
+    p.args.lanes = 32;
+    while (p.args.lanes / 2 >= v && p.args.lanes > 1) p.args.lanes /= 2;
+    p.cpt = v <= 32 ? 1 : v <= 64 ? 2 : 4;
+    p.args.warps_per_row = 1;
+    while (p.args.warps_per_row * 32 * p.cpt < v) p.args.warps_per_row *= 2;
+    return p;
+}
+// Stages of `stage` bytes that fit in `room` bytes, two at least.
+int stages_in(std::size_t room, std::size_t stage) {
+    const std::size_t fit = room / stage;
+    return static_cast<int>(fit < 2 ? 2 : fit < ring_kernels::kMaxStages ? fit : ring_kernels::kMaxStages);
+}
+
+RingPlan plan_forward_ring(std::size_t rows, std::size_t hidden, std::size_t elem, bool fused) {
+    RingPlan p = plan_ring_common(hidden, elem);
+    auto& a = p.args;
+    a.step_rows = a.warps_per_row > 1 ? 1 : ring_kernels::kLaneVectors / p.cpt * (32 / a.lanes);
+    a.data_offset = ring_kernels::kVectorsOffset + static_cast<unsigned>(2 * hidden * sizeof(float));
+    const std::size_t stage = a.step_rows * hidden * elem * (fused ? 2 : 1), room = kSmemPerSm - a.data_offset;
+    // As many row groups as threads and two stages each allow, fewer when there are few rows: then every SM gets some.
+    std::size_t groups = (fused ? ring_kernels::kFusedThreads : ring_kernels::kForwardThreads) / 32 / a.warps_per_row;
+    const std::size_t fit = room / (2 * stage), share = (rows + static_cast<std::size_t>(kNumSMs) * a.step_rows - 1) / (static_cast<std::size_t>(kNumSMs) * a.step_rows);
+    groups = groups < fit ? groups : fit;
+    groups = groups < share ? groups : share;
+    a.groups = static_cast<int>(groups);
+    a.stages = stages_in(room / groups, stage);
+    p.smem = a.data_offset + groups * a.stages * stage;
+    p.threads = a.groups * a.warps_per_row * 32;
+    const std::size_t need = (rows + groups * a.step_rows - 1) / (groups * a.step_rows);
+    p.grid = static_cast<unsigned>(need < kNumSMs ? need : kNumSMs);
+    return p;
+}
+
+RingPlan plan_backward_ring(std::size_t rows, std::size_t hidden, std::size_t elem) {
+    RingPlan p = plan_ring_common(hidden, elem);
+    auto& a = p.args;
+    const std::size_t v = a.vectors;
+    p.threads = v <= 256 ? 256 : ring_kernels::kBackwardThreads;
+    p.cols = v <= 512 ? 1 : v <= 1024 ? 2 : 4;
+    const std::size_t ctas = ring_kernels::kBackwardThreads / p.threads, rows_each = ring_kernels::kLaneVectors / p.cols;
+    std::size_t groups = p.cols == 1 ? p.threads / v : 1;
+    const std::size_t most = ring_kernels::kMaxTileRows / rows_each, share = (rows + kNumSMs * ctas * rows_each - 1) / (kNumSMs * ctas * rows_each);
+    groups = groups < most ? groups : most;
+    groups = groups < share ? groups : share;
+    a.groups = static_cast<int>(groups);
+    a.step_rows = static_cast<int>(groups * rows_each);
+    a.data_offset = ring_kernels::kVectorsOffset + static_cast<unsigned>(hidden * sizeof(float));
+    const std::size_t stage = 2 * a.step_rows * hidden * elem;
+    a.stages = stages_in(kSmemPerSm / ctas - 10 * 1024 - a.data_offset, stage);
+    p.smem = a.data_offset + a.stages * stage;
+    const std::size_t need = (rows + a.step_rows - 1) / a.step_rows, cap = kNumSMs * ctas;
     p.grid = static_cast<unsigned>(need < cap ? need : cap);
     return p;
 }
@@ -233,37 +352,61 @@ bool valid_rows(std::size_t rows, std::size_t hidden) {
     return rows != 0 && hidden != 0 && hidden <= 0x7fffffffull && rows <= (1ull << 46) / hidden;
 }
 
+template <typename Kernel>
+int allow_smem(Kernel kernel, PerDeviceOnce* once) {
+    if (once->needed()) {
+        cudaFuncAttributes a;
+        CGPT_CUDA_TRY(cudaFuncGetAttributes(&a, kernel));
+        CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - static_cast<int>(a.sharedSizeBytes)));
+        once->done();
+    }
+    return CGPT_OK;
+}
+
 // Enough for the call's layout whatever its type and alignment turn out to be.
 std::size_t workspace_bytes(std::size_t rows, std::size_t hidden) {
     std::size_t parts = 0, stats = 0;
     for (std::size_t elem : {2, 4})
         for (bool vector : {false, true}) {
-            const Plan p = make_plan(rows, hidden, elem, vector);
-            const std::size_t n = p.vec != 0 ? p.grid : any_splits(rows);
+            const Form form = form_of(hidden, elem, vector);
+            const std::size_t n = form == Form::kRing ? plan_backward_ring(rows, hidden, elem).grid
+                                  : form == Form::kRows ? plan_rows(rows, hidden).grid : any_splits(rows);
             if (n > parts) parts = n;
-            if (p.vec == 0) stats = rows * sizeof(float2);
+            if (form == Form::kAny) stats = rows * sizeof(float2);
         }
     return parts * 2 * hidden * sizeof(float) + stats;
 }
 
-// Calls `f` with the plan's vector width, vectors per thread and rows at a time as compile-time constants.
-template <typename T, typename F>
-int with_layout(const Plan& p, F f) {
-    constexpr int V = 16 / sizeof(T);
-#define CGPT_LAYOUT(VEC, CPT, R) f(std::integral_constant<int, VEC>{}, std::integral_constant<int, CPT>{}, std::integral_constant<int, R>{})
-    if (p.vec == V) return p.cpt == 1 ? CGPT_LAYOUT(V, 1, 4) : p.cpt == 2 ? CGPT_LAYOUT(V, 2, 2) : CGPT_LAYOUT(V, 4, 1);
-    return p.cpt == 4 ? CGPT_LAYOUT(1, 4, 2) : CGPT_LAYOUT(1, 16, 1);
-#undef CGPT_LAYOUT
-}
+template <int N> using Int = std::integral_constant<int, N>;
 
 template <typename T, bool FUSED>
 int launch_forward(void* y, void* sum, const void* x, const void* residual, const void* w, const void* b, std::size_t rows,
                    std::size_t hidden, float epsilon, const DropoutArgs& args, cudaStream_t s) {
     const bool al = aligned16(y) && aligned16(sum) && aligned16(x) && aligned16(residual) && aligned16(w) && aligned16(b);
-    const Plan p = make_plan(rows, hidden, sizeof(T), al);
-    if (p.vec != 0)
-        return with_layout<T>(p, [&](auto vec, auto cpt, auto r) {
-            auto kernel = rows_kernels::layernorm_forward_rows_kernel<T, vec.value, cpt.value, r.value, FUSED>;
+    const Form form = form_of(hidden, sizeof(T), al);
+    if (form == Form::kRing) {
+        const RingPlan p = plan_forward_ring(rows, hidden, sizeof(T), FUSED);
+        auto launch = [&](auto cpt) {
+            auto kernel = ring_kernels::layernorm_forward_ring_kernel<T, cpt.value, FUSED>;
+            static PerDeviceOnce once;
+            CGPT_TRY(allow_smem(kernel, &once));
+            auto args_on_device = p.args;
+            args_on_device.status = tc_status_device_ptr();
+            if (args_on_device.status == nullptr) return CGPT_ERR_STATE;
+            kernel<<<p.grid, p.threads, p.smem, s>>>(
+                static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
+                static_cast<const T*>(w), static_cast<const T*>(b), static_cast<long long>(rows), static_cast<int>(hidden), epsilon,
+                args_on_device, args);
+            count_launch();
+            CGPT_LAUNCH_CHECK();
+            return CGPT_OK;
+        };
+        return p.cpt == 1 ? launch(Int<1>{}) : p.cpt == 2 ? launch(Int<2>{}) : launch(Int<4>{});
+    }
+    if (form == Form::kRows) {
+        const RowsPlan p = plan_rows(rows, hidden);
+        auto launch = [&](auto cpt, auto r) {
+            auto kernel = rows_kernels::layernorm_forward_rows_kernel<T, cpt.value, r.value, FUSED>;
             const int threads = p.groups * p.tpr;
             const std::size_t at_once = static_cast<std::size_t>(p.groups) * r.value, need = (rows + at_once - 1) / at_once;
             const std::size_t cap = static_cast<std::size_t>(kNumSMs) * resident_ctas_per_sm(reinterpret_cast<const void*>(kernel), threads, 0);
@@ -274,7 +417,9 @@ int launch_forward(void* y, void* sum, const void* x, const void* residual, cons
             count_launch();
             CGPT_LAUNCH_CHECK();
             return CGPT_OK;
-        });
+        };
+        return p.cpt == 4 ? launch(Int<4>{}, Int<2>{}) : launch(Int<16>{}, Int<1>{});
+    }
     layernorm_forward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
         static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
         static_cast<const T*>(w), static_cast<const T*>(b), static_cast<long long>(rows), static_cast<long long>(hidden), epsilon, args);
@@ -296,20 +441,42 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
         return CGPT_OK;
     };
     const bool al = aligned16(dx) && aligned16(din) && aligned16(dy) && aligned16(x) && aligned16(w) && aligned16(residual);
-    const Plan p = make_plan(rows, hidden, sizeof(T), al);
-    if (p.vec != 0)
-        return with_layout<T>(p, [&](auto vec, auto cpt, auto r) {
-            const std::size_t sums = static_cast<std::size_t>(p.groups) * 4 * r.value * 16 * sizeof(float);
-            const std::size_t parts = p.groups > 1 ? static_cast<std::size_t>(2) * cpt.value * vec.value * p.tpr * sizeof(float) : 0;
-            rows_kernels::layernorm_backward_rows_kernel<T, vec.value, cpt.value, r.value, FUSED>
-                <<<p.grid, p.groups * p.tpr, sums > parts ? sums : parts, s>>>(
-                    static_cast<T*>(dx), static_cast<T*>(din), partial, static_cast<const T*>(dy), static_cast<const T*>(x),
-                    static_cast<const T*>(w), static_cast<const T*>(residual), static_cast<long long>(rows), static_cast<int>(hidden),
-                    epsilon, p.tpr, args);
+    const Form form = form_of(hidden, sizeof(T), al);
+    if (form == Form::kRing) {
+        const RingPlan p = plan_backward_ring(rows, hidden, sizeof(T));
+        auto launch = [&](auto cpt, auto cols) {
+            auto kernel = ring_kernels::layernorm_backward_ring_kernel<T, cpt.value, cols.value, FUSED>;
+            static PerDeviceOnce once;
+            CGPT_TRY(allow_smem(kernel, &once));
+            auto args_on_device = p.args;
+            args_on_device.status = tc_status_device_ptr();
+            if (args_on_device.status == nullptr) return CGPT_ERR_STATE;
+            kernel<<<p.grid, p.threads, p.smem, s>>>(
+                static_cast<T*>(dx), static_cast<T*>(din), partial, static_cast<const T*>(dy), static_cast<const T*>(x),
+                static_cast<const T*>(w), static_cast<const T*>(residual), static_cast<long long>(rows), static_cast<int>(hidden),
+                epsilon, args_on_device, args);
             count_launch();
             CGPT_LAUNCH_CHECK();
             return reduce(p.grid);
-        });
+        };
+        if (p.cols == 1) return p.cpt == 1 ? launch(Int<1>{}, Int<1>{}) : p.cpt == 2 ? launch(Int<2>{}, Int<1>{}) : launch(Int<4>{}, Int<1>{});
+        return p.cols == 2 ? launch(Int<4>{}, Int<2>{}) : launch(Int<4>{}, Int<4>{});
+    }
+    if (form == Form::kRows) {
+        const RowsPlan p = plan_rows(rows, hidden);
+        auto launch = [&](auto cpt, auto r) {
+            const std::size_t sums = static_cast<std::size_t>(p.groups) * 4 * r.value * 16 * sizeof(float);
+            const std::size_t parts = static_cast<std::size_t>(2) * cpt.value * p.tpr * sizeof(float);
+            rows_kernels::layernorm_backward_rows_kernel<T, cpt.value, r.value, FUSED><<<p.grid, p.groups * p.tpr, sums > parts ? sums : parts, s>>>(
+                static_cast<T*>(dx), static_cast<T*>(din), partial, static_cast<const T*>(dy), static_cast<const T*>(x),
+                static_cast<const T*>(w), static_cast<const T*>(residual), static_cast<long long>(rows), static_cast<int>(hidden),
+                epsilon, p.tpr, args);
+            count_launch();
+            CGPT_LAUNCH_CHECK();
+            return reduce(p.grid);
+        };
+        return p.cpt == 4 ? launch(Int<4>{}, Int<2>{}) : launch(Int<16>{}, Int<1>{});
+    }
     const std::size_t splits = any_splits(rows);
     float2* stats = reinterpret_cast<float2*>(partial + splits * 2 * hidden);
     layernorm_backward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
