@@ -248,13 +248,16 @@ layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __r
 // the fused operators give the bits of their parts.
 enum class Form { kAny, kRows, kRing };
 
-constexpr std::size_t kSmemPerSm = 222 * 1024;   // what the resident CTAs of an SM share, less what the hardware keeps
+constexpr std::size_t kSmemPerSm = 227 * 1024;
 
-// Rings take rows of which shared memory holds two stages of both tensors of the fused forward beside w and b (14016 16-bit
-// or 8192 fp32 elements).
+// Where the rings begin behind `vectors` fp32 vectors.
+std::size_t vectors_end(std::size_t hidden, std::size_t vectors) { return ring_kernels::kVectorsOffset + (vectors * hidden * sizeof(float) + 127) / 128 * 128; }
+
+// Rings take rows of which shared memory holds two stages of both tensors of the fused forward beside w and b, and of which a
+// CTA of the backward holds a row (14 k 16-bit or 8192 fp32 elements).
 Form form_of(std::size_t hidden, std::size_t elem, bool vector) {
     if (vector && hidden * elem % 16 == 0)
-        return hidden * elem / 16 <= 2048 && ring_kernels::kVectorsOffset + 2 * hidden * sizeof(float) + 4 * hidden * elem <= kSmemPerSm ? Form::kRing : Form::kAny;
+        return hidden * elem / 16 <= ring_kernels::kTileVectors * ring_kernels::kBackwardThreads && vectors_end(hidden, 2) + 4 * hidden * elem <= kSmemPerSm ? Form::kRing : Form::kAny;
     return hidden <= 16 * rows_kernels::kMaxTpr ? Form::kRows : Form::kAny;
 }
 
@@ -277,66 +280,63 @@ RowsPlan plan_rows(std::size_t rows, std::size_t hidden) {
 struct RingPlan {
     ring_kernels::RingArgs args;
     int cpt, cols, threads;
+    bool full;        // the lanes of a row hold exactly its vectors
     unsigned grid;
     std::size_t smem;
 };
 
-RingPlan plan_ring_common(std::size_t hidden, std::size_t elem) {
+// Lanes and warps of a row whose lanes hold up to most_cpt vectors.
+RingPlan plan_row(std::size_t hidden, std::size_t elem, int most_cpt) {
     RingPlan p{};
-    const int v = static_cast<int>(hidden * elem / 16);
-    p.args.vectors = v;
-    p.args.lanes = 32;
-    while (p.args.lanes / 2 >= v && p.args.lanes > 1) p.args.lanes /= 2;
-    p.cpt = v <= 32 ? 1 : v <= 64 ? 2 : 4;
-    p.args.warps_per_row = 1;
-    while (p.args.warps_per_row * 32 * p.cpt < v) p.args.warps_per_row *= 2;
-    return p;
-}
-// Stages of `stage` bytes that fit in `room` bytes, two at least.
-int stages_in(std::size_t room, std::size_t stage) {
-    const std::size_t fit = room / stage;
-    return static_cast<int>(fit < 2 ? 2 : fit < ring_kernels::kMaxStages ? fit : ring_kernels::kMaxStages);
-}
-
-RingPlan plan_forward_ring(std::size_t rows, std::size_t hidden, std::size_t elem, bool fused) {
-    RingPlan p = plan_ring_common(hidden, elem);
     auto& a = p.args;
-    a.step_rows = a.warps_per_row > 1 ? 1 : ring_kernels::kLaneVectors / p.cpt * (32 / a.lanes);
-    a.data_offset = ring_kernels::kVectorsOffset + static_cast<unsigned>(2 * hidden * sizeof(float));
+    const int v = static_cast<int>(hidden * elem / 16);
+    a.vectors = v;
+    a.lanes = 32;
+    while (a.lanes / 2 >= v && a.lanes > 1) a.lanes /= 2;
+    p.cpt = 1;
+    while (p.cpt < most_cpt && 32 * p.cpt < v) p.cpt *= 2;
+    a.warps_per_row = 1;
+    while (a.warps_per_row * 32 * p.cpt < v) a.warps_per_row *= 2;
+    p.full = a.warps_per_row * a.lanes * p.cpt == v;
+    return p;
+}
+std::size_t at_most(std::size_t n, std::size_t limit) { return n < limit ? n : limit; }
+std::size_t over(std::size_t n, std::size_t d) { return (n + d - 1) / d; }
+
+// As many groups as threads and two stages each allow, fewer when there are few rows: then every SM gets some.
+RingPlan plan_forward_ring(std::size_t rows, std::size_t hidden, std::size_t elem, bool fused) {
+    RingPlan p = plan_row(hidden, elem, 8);
+    auto& a = p.args;
+    a.step_rows = ring_kernels::rows_at_once(p.cpt) * (32 / a.lanes);
+    a.data_offset = static_cast<unsigned>(vectors_end(hidden, 2));
     const std::size_t stage = a.step_rows * hidden * elem * (fused ? 2 : 1), room = kSmemPerSm - a.data_offset;
-    // As many row groups as threads and two stages each allow, fewer when there are few rows: then every SM gets some.
-    std::size_t groups = (fused ? ring_kernels::kFusedThreads : ring_kernels::kForwardThreads) / 32 / a.warps_per_row;
-    const std::size_t fit = room / (2 * stage), share = (rows + static_cast<std::size_t>(kNumSMs) * a.step_rows - 1) / (static_cast<std::size_t>(kNumSMs) * a.step_rows);
-    groups = groups < fit ? groups : fit;
-    groups = groups < share ? groups : share;
+    std::size_t groups = ring_kernels::kForwardThreads / 32 / a.warps_per_row;
+    groups = at_most(at_most(groups, room / (2 * stage)), over(rows, static_cast<std::size_t>(kNumSMs) * a.step_rows));
     a.groups = static_cast<int>(groups);
-    a.stages = stages_in(room / groups, stage);
-    p.smem = a.data_offset + groups * a.stages * stage;
+    a.stages = static_cast<int>(at_most(room / groups / stage, ring_kernels::kMaxStages));
     p.threads = a.groups * a.warps_per_row * 32;
-    const std::size_t need = (rows + groups * a.step_rows - 1) / (groups * a.step_rows);
-    p.grid = static_cast<unsigned>(need < kNumSMs ? need : kNumSMs);
+    p.smem = a.data_offset + groups * a.stages * stage;
+    p.grid = static_cast<unsigned>(at_most(over(rows, groups * a.step_rows), kNumSMs));
     return p;
 }
 
+// Threads cover as many rows at a time as they have vectors for, fewer when there are few rows.
 RingPlan plan_backward_ring(std::size_t rows, std::size_t hidden, std::size_t elem) {
-    RingPlan p = plan_ring_common(hidden, elem);
+    RingPlan p = plan_row(hidden, elem, 4);
     auto& a = p.args;
     const std::size_t v = a.vectors;
     p.threads = v <= 256 ? 256 : ring_kernels::kBackwardThreads;
     p.cols = v <= 512 ? 1 : v <= 1024 ? 2 : 4;
-    const std::size_t ctas = ring_kernels::kBackwardThreads / p.threads, rows_each = ring_kernels::kLaneVectors / p.cols;
+    const std::size_t ctas = ring_kernels::kBackwardThreads / p.threads, rows_each = ring_kernels::kTileVectors / p.cols;
     std::size_t groups = p.cols == 1 ? p.threads / v : 1;
-    const std::size_t most = ring_kernels::kMaxTileRows / rows_each, share = (rows + kNumSMs * ctas * rows_each - 1) / (kNumSMs * ctas * rows_each);
-    groups = groups < most ? groups : most;
-    groups = groups < share ? groups : share;
+    groups = at_most(at_most(groups, ring_kernels::kMaxTileRows / rows_each), over(rows, kNumSMs * ctas * rows_each));
     a.groups = static_cast<int>(groups);
     a.step_rows = static_cast<int>(groups * rows_each);
-    a.data_offset = ring_kernels::kVectorsOffset + static_cast<unsigned>(hidden * sizeof(float));
-    const std::size_t stage = 2 * a.step_rows * hidden * elem;
-    a.stages = stages_in(kSmemPerSm / ctas - 10 * 1024 - a.data_offset, stage);
+    a.data_offset = static_cast<unsigned>(vectors_end(hidden, 1));
+    const std::size_t stage = 2 * a.step_rows * hidden * elem, fixed = ring_kernels::kStatsBytes + 1024;   // 1024: kept by the hardware
+    a.stages = static_cast<int>(at_most((kSmemPerSm + 1024) / ctas - fixed - a.data_offset, ring_kernels::kMaxStages * stage) / stage);
     p.smem = a.data_offset + a.stages * stage;
-    const std::size_t need = (rows + a.step_rows - 1) / a.step_rows, cap = kNumSMs * ctas;
-    p.grid = static_cast<unsigned>(need < cap ? need : cap);
+    p.grid = static_cast<unsigned>(at_most(over(rows, a.step_rows), kNumSMs * ctas));
     return p;
 }
 
@@ -353,11 +353,9 @@ bool valid_rows(std::size_t rows, std::size_t hidden) {
 }
 
 template <typename Kernel>
-int allow_smem(Kernel kernel, PerDeviceOnce* once) {
+int allow_smem(Kernel kernel, PerDeviceOnce* once, std::size_t fixed = 0) {
     if (once->needed()) {
-        cudaFuncAttributes a;
-        CGPT_CUDA_TRY(cudaFuncGetAttributes(&a, kernel));
-        CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - static_cast<int>(a.sharedSizeBytes)));
+        CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemPerSm - fixed)));
         once->done();
     }
     return CGPT_OK;
@@ -386,8 +384,8 @@ int launch_forward(void* y, void* sum, const void* x, const void* residual, cons
     const Form form = form_of(hidden, sizeof(T), al);
     if (form == Form::kRing) {
         const RingPlan p = plan_forward_ring(rows, hidden, sizeof(T), FUSED);
-        auto launch = [&](auto cpt) {
-            auto kernel = ring_kernels::layernorm_forward_ring_kernel<T, cpt.value, FUSED>;
+        auto launch = [&](auto cpt, auto full) {
+            auto kernel = ring_kernels::layernorm_forward_ring_kernel<T, cpt.value, full.value, FUSED>;
             static PerDeviceOnce once;
             CGPT_TRY(allow_smem(kernel, &once));
             auto args_on_device = p.args;
@@ -401,7 +399,8 @@ int launch_forward(void* y, void* sum, const void* x, const void* residual, cons
             CGPT_LAUNCH_CHECK();
             return CGPT_OK;
         };
-        return p.cpt == 1 ? launch(Int<1>{}) : p.cpt == 2 ? launch(Int<2>{}) : launch(Int<4>{});
+        auto either = [&](auto cpt) { return p.full ? launch(cpt, std::true_type{}) : launch(cpt, std::false_type{}); };
+        return p.cpt == 1 ? either(Int<1>{}) : p.cpt == 2 ? either(Int<2>{}) : p.cpt == 4 ? either(Int<4>{}) : either(Int<8>{});
     }
     if (form == Form::kRows) {
         const RowsPlan p = plan_rows(rows, hidden);
@@ -444,10 +443,10 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
     const Form form = form_of(hidden, sizeof(T), al);
     if (form == Form::kRing) {
         const RingPlan p = plan_backward_ring(rows, hidden, sizeof(T));
-        auto launch = [&](auto cpt, auto cols) {
-            auto kernel = ring_kernels::layernorm_backward_ring_kernel<T, cpt.value, cols.value, FUSED>;
+        auto launch = [&](auto cpt, auto cols, auto full) {
+            auto kernel = ring_kernels::layernorm_backward_ring_kernel<T, cpt.value, cols.value, full.value, FUSED>;
             static PerDeviceOnce once;
-            CGPT_TRY(allow_smem(kernel, &once));
+            CGPT_TRY(allow_smem(kernel, &once, ring_kernels::kStatsBytes));
             auto args_on_device = p.args;
             args_on_device.status = tc_status_device_ptr();
             if (args_on_device.status == nullptr) return CGPT_ERR_STATE;
@@ -459,8 +458,9 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
             CGPT_LAUNCH_CHECK();
             return reduce(p.grid);
         };
-        if (p.cols == 1) return p.cpt == 1 ? launch(Int<1>{}, Int<1>{}) : p.cpt == 2 ? launch(Int<2>{}, Int<1>{}) : launch(Int<4>{}, Int<1>{});
-        return p.cols == 2 ? launch(Int<4>{}, Int<2>{}) : launch(Int<4>{}, Int<4>{});
+        auto either = [&](auto cpt, auto cols) { return p.full ? launch(cpt, cols, std::true_type{}) : launch(cpt, cols, std::false_type{}); };
+        if (p.cols == 1) return p.cpt == 1 ? either(Int<1>{}, Int<1>{}) : p.cpt == 2 ? either(Int<2>{}, Int<1>{}) : either(Int<4>{}, Int<1>{});
+        return p.cols == 2 ? either(Int<4>{}, Int<2>{}) : either(Int<4>{}, Int<4>{});
     }
     if (form == Form::kRows) {
         const RowsPlan p = plan_rows(rows, hidden);

@@ -5,23 +5,27 @@
 //  * rows come through rings of stages in shared memory, filled by bulk copies (consecutive rows are contiguous: one copy per
 //    tensor and stage), so that nothing but one thread per ring deals with memory and its latency;
 //  * arithmetic is on pairs (fma / mul / add .f32x2): one issue slot for two elements;
-//  * a row is summed by one warp wherever 128 vectors hold it, four vectors per lane: the shuffles of a sum are shared by up to
-//    32 elements of a lane, and by up to four rows where rows are short;
-//  * w and b are kept in shared memory as fp32: no conversion per row.
+//  * a row is summed by as few warps as hold it in registers, so that the shuffles of a sum are shared by up to 64 elements of a
+//    lane, and by up to four rows where rows are short; what is read is converted to fp32 once;
+//  * w and b are kept in shared memory as fp32: no conversion per row;
 //
 // Forward: every group of warps walks rows through a ring of its own. Backward: a CTA takes tiles of rows in two phases, rows
 // first (a warp group per row: mean, rstd and the two sums of dx, left in shared memory), then columns (a thread per vector of
-// columns: dx, and the running dw and db of its columns in registers).
+// columns: dx, and the running dw and db of its columns in registers). Lanes that keep both a row's values and dw and db of
+// their columns need 168 registers, and 12 warps an SM hide less: measured 62 against 57 us at 16384 x 2048 bf16.
 #pragma once
 
 namespace ring_kernels {
 
 constexpr int kMaxStages = 4;
-constexpr int kLaneVectors = 4;          // vectors of a row step that a lane holds: CPT vectors of R = 4 / CPT rows
-constexpr int kForwardThreads = 1024;    // one CTA per SM (64 registers)
-constexpr int kFusedThreads = 640;       // the fused forward needs up to 96
-constexpr int kBackwardThreads = 512;    // per SM: two CTAs of 256 or one of 512 (128 registers)
-constexpr int kMaxTileRows = 256;
+constexpr int kForwardThreads = 512;     // one CTA per SM (128 registers)
+constexpr int kBackwardThreads = 512;    // per SM: two CTAs of 256, or one of 512 for rows of more than 256 vectors
+constexpr int kTileVectors = 4;          // vectors of each tensor that a thread of the backward takes per tile
+constexpr int kMaxTileRows = 128;
+constexpr std::size_t kStatsBytes = 2 * kMaxTileRows * 32;   // static shared memory of the backward
+
+// Rows a warp group takes at a time: a lane with few vectors per row holds several rows.
+__host__ __device__ constexpr int rows_at_once(int cpt) { return cpt >= 4 ? 1 : 4 / cpt; }
 
 using Pair = unsigned long long;         // two fp32 values in a 64-bit register
 
@@ -113,10 +117,6 @@ __device__ __forceinline__ void drop_pairs(Pair (&p)[8 / sizeof(T)], const Philo
     for (int i = 0; i < VEC / 2; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
 }
 
-// Makes packed values opaque to the optimiser, so that it converts them again at their next use instead of keeping twice as many
-// fp32 registers alive from one use to the next.
-__device__ __forceinline__ void keep_packed(uint4& v) { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }
-
 // A ring of stages. A wait that runs out sets the library's status word; the CTA then goes on with what is there (every barrier
 // is still met, nothing is written out of bounds) and waits no more.
 struct Ring {
@@ -132,14 +132,16 @@ struct Ring {
         for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[s], 1);
         sm100::mbar_init_fence();
     }
-    // Rows row0 .. row0 + step_rows of a and b (b may be null) into stage s, as far as there are such rows.
+    // Rows row0 .. row0 + step_rows of a, b and c (b and c may be null) into stage s, as far as there are such rows.
     template <typename T>
-    __device__ __forceinline__ void fill(int s, const T* a, const T* b, long long row0, int step_rows, long long rows, int hidden) const {
+    __device__ __forceinline__ void fill(int s, const T* a, const T* b, const T* c, long long row0, int step_rows, long long rows, int hidden) const {
         if (row0 >= rows) return;
         const unsigned n = static_cast<unsigned>(rows - row0 < step_rows ? rows - row0 : step_rows) * row_bytes;
-        sm100::mbar_expect_tx(&full[s], b != nullptr ? 2 * n : n);
-        sm100::bulk_load_1d(data + s * stage_bytes, a + row0 * hidden, n, &full[s]);
-        if (b != nullptr) sm100::bulk_load_1d(data + s * stage_bytes + tensor_bytes, b + row0 * hidden, n, &full[s]);
+        unsigned char* to = data + s * stage_bytes;
+        sm100::mbar_expect_tx(&full[s], (1 + (b != nullptr) + (c != nullptr)) * n);
+        sm100::bulk_load_1d(to, a + row0 * hidden, n, &full[s]);
+        if (b != nullptr) sm100::bulk_load_1d(to + tensor_bytes, b + row0 * hidden, n, &full[s]);
+        if (c != nullptr) sm100::bulk_load_1d(to + 2 * tensor_bytes, c + row0 * hidden, n, &full[s]);
     }
     __device__ __forceinline__ const unsigned char* wait() {
         if (!failed && !sm100::mbar_wait(&full[stage], parity)) {
@@ -153,12 +155,12 @@ struct Ring {
     }
 };
 
-// Layout of a launch (make_ring_plan): vectors per row, lanes per row (fewer than 32 where a warp holds several rows), warps
-// per row, rows a step or tile has, groups (forward: warp groups; backward: row groups of the column phase).
+// Layout of a launch: vectors per row, lanes per row (fewer than 32 where a warp holds several rows), warps per row, rows a group
+// of such warps takes at a time, groups in a CTA, stages of each group's ring.
 struct RingArgs {
     unsigned int* status;
     int vectors, lanes, warps_per_row, step_rows, groups, stages;
-    unsigned data_offset;               // of the ring(s) in shared memory
+    unsigned data_offset;               // of the rings in shared memory
 };
 
 // Totals of N values over the `lanes` lanes (a power of two) of a row.
@@ -196,7 +198,8 @@ __device__ __forceinline__ void warps_sum(float (&v)[N], int warps, int warp, in
     }
 }
 
-// w or b (null: zeros) as fp32 in shared memory.
+// w or b (null: zeros) as fp32 in shared memory, four values at a time: the lanes that read consecutive vectors of eight find
+// their first halves side by side in one area and their second halves in the next (no bank conflicts).
 template <typename T>
 __device__ __forceinline__ void stage_vector(float* to, const T* from, int vectors) {
     constexpr int VEC = 16 / sizeof(T), NP = VEC / 2;
@@ -204,36 +207,37 @@ __device__ __forceinline__ void stage_vector(float* to, const T* from, int vecto
         Pair v[NP];
         to_pairs<T>(v, from != nullptr ? *reinterpret_cast<const uint4*>(from + i * VEC) : make_uint4(0u, 0u, 0u, 0u));
 #pragma unroll
-        for (int j = 0; j < NP / 2; ++j) reinterpret_cast<ulonglong2*>(to + i * VEC)[j] = make_ulonglong2(v[2 * j], v[2 * j + 1]);
+        for (int j = 0; j < NP / 2; ++j) reinterpret_cast<ulonglong2*>(to)[j * vectors + i] = make_ulonglong2(v[2 * j], v[2 * j + 1]);
     }
 }
 template <int NP>
-__device__ __forceinline__ void read_pairs(Pair (&p)[NP], const float* from) {
-    const ulonglong2* v = reinterpret_cast<const ulonglong2*>(from);
+__device__ __forceinline__ void read_pairs(Pair (&p)[NP], const float* from, int vec, int vectors) {
 #pragma unroll
-    for (int i = 0; i < NP / 2; ++i) {
-        const ulonglong2 u = v[i];
-        p[2 * i] = u.x;
-        p[2 * i + 1] = u.y;
+    for (int j = 0; j < NP / 2; ++j) {
+        const ulonglong2 u = reinterpret_cast<const ulonglong2*>(from)[j * vectors + vec];
+        p[2 * j] = u.x;
+        p[2 * j + 1] = u.y;
     }
 }
 
-// Shared memory: [barriers 1 KB][sums of multi-warp rows 2 KB][w][b][rings]
-constexpr unsigned kSumsOffset = 1024, kVectorsOffset = 3072;
+// Shared memory: [barriers][sums of multi-warp rows: 64 floats per group][w][b (forward)][rings]
+constexpr int kMaxGroups = 16;                     // at most half as many where a row takes several warps
+constexpr unsigned kSumsOffset = kMaxGroups * kMaxStages * 8, kVectorsOffset = kSumsOffset + kMaxGroups / 2 * 64 * 4;
 
-template <typename T, int CPT, bool FUSED>
-__global__ void __launch_bounds__(FUSED ? kFusedThreads : kForwardThreads, 1)
+// FULL: the lanes of a row hold exactly its vectors, so that no column is checked.
+template <typename T, int CPT, bool FULL, bool FUSED>
+__global__ void __launch_bounds__(kForwardThreads, 1)
 layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* residual, const T* __restrict__ w, const T* __restrict__ b,
                               long long rows, int hidden, float epsilon, const RingArgs ra, const DropoutArgs args) {
-    constexpr int VEC = 16 / sizeof(T), NP = VEC / 2, R = kLaneVectors / CPT;
+    constexpr int VEC = 16 / sizeof(T), NP = VEC / 2, R = rows_at_once(CPT);
     extern __shared__ __align__(128) unsigned char shared[];
     float* ws = reinterpret_cast<float*>(shared + kVectorsOffset);
     float* bs = ws + hidden;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = warp / ra.warps_per_row, warp_in_row = warp - group * ra.warps_per_row;
     const int per_warp = 32 / ra.lanes;                      // rows side by side in a warp
-    const int lane_row = lane / ra.lanes, vec0 = warp_in_row * 32 + (lane & (ra.lanes - 1)), vec_step = ra.warps_per_row * ra.lanes;
-    float* red = reinterpret_cast<float*>(shared + kSumsOffset) + group * 32;
+    const int lane_row = lane / ra.lanes, vec0 = warp_in_row * (32 * CPT) + (lane & (ra.lanes - 1));
+    float* red = reinterpret_cast<float*>(shared + kSumsOffset) + group * 64;
     const long long step = static_cast<long long>(gridDim.x) * ra.groups * ra.step_rows;
     const long long first = (static_cast<long long>(blockIdx.x) * ra.groups + group) * ra.step_rows;
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
@@ -246,102 +250,93 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
     ring.full = reinterpret_cast<std::uint64_t*>(shared) + group * kMaxStages;
     ring.data = shared + ra.data_offset + static_cast<std::size_t>(group) * ra.stages * ring.stage_bytes;
     ring.status = ra.status;
-    const T* second = FUSED ? residual : nullptr;
+    const T *second = FUSED ? residual : nullptr, *none = nullptr;
     if (leader) {
         ring.init();
-        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, second, first + s * step, ra.step_rows, rows, hidden);
+        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, second, none, first + s * step, ra.step_rows, rows, hidden);
     }
     stage_vector(ws, w, ra.vectors);
     stage_vector(bs, b, ra.vectors);
     const Philox gen(args);
+    const unsigned lane_bytes = lane_row * ring.row_bytes + vec0 * 16, next_row = per_warp * ring.row_bytes;
     __syncthreads();
 
     for (long long row0 = first; row0 < rows; row0 += step) {
-        const unsigned char* stage = ring.wait();
-        uint4 xp[R][CPT];
+        const unsigned char* at = ring.wait() + lane_bytes;
+        const int left = rows - row0 < ra.step_rows ? static_cast<int>(rows - row0) : ra.step_rows;   // rows of this step
+        const long long e0 = (row0 + lane_row) * hidden + vec0 * VEC;                                 // the lane's first element
+        Pair v[R][CPT][NP];
         float mean[R], rstd[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int in_step = r * per_warp + lane_row;
             Pair acc = 0;
 #pragma unroll
             for (int c = 0; c < CPT; ++c) {
-                const int vec = vec0 + c * vec_step;
-                const bool in = row0 + in_step < rows && vec < ra.vectors;
-                xp[r][c] = make_uint4(0u, 0u, 0u, 0u);      // a stage keeps what an earlier step left there
-                if (in) {
-                    xp[r][c] = *reinterpret_cast<const uint4*>(stage + in_step * ring.row_bytes + vec * 16);
-                    Pair v[NP];
-                    to_pairs<T>(v, xp[r][c]);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) v[r][c][i] = 0;         // a stage keeps what an earlier step left there
+                if ((R == 1 || r * per_warp + lane_row < left) && (FULL || vec0 + c * 32 < ra.vectors)) {
+                    to_pairs<T>(v[r][c], *reinterpret_cast<const uint4*>(at + r * next_row + c * 512));
                     if constexpr (FUSED) {
-                        const long long e = (row0 + in_step) * hidden + vec * VEC;
-                        if (args.threshold != 0) drop_pairs<T>(v, gen, e, args);
+                        const long long e = e0 + r * per_warp * hidden + c * (32 * VEC);
+                        if (args.threshold != 0) drop_pairs<T>(v[r][c], gen, e, args);
                         Pair res[NP];
-                        to_pairs<T>(res, *reinterpret_cast<const uint4*>(stage + ring.tensor_bytes + in_step * ring.row_bytes + vec * 16));
+                        to_pairs<T>(res, *reinterpret_cast<const uint4*>(at + ring.tensor_bytes + r * next_row + c * 512));
 #pragma unroll
-                        for (int i = 0; i < NP; ++i) v[i] = add2(v[i], res[i]);
-                        xp[r][c] = to_raw<T>(v);
-                        *reinterpret_cast<uint4*>(sum + e) = xp[r][c];
-                        to_pairs<T>(v, xp[r][c]);            // the norm is of the stored value
+                        for (int i = 0; i < NP; ++i) v[r][c][i] = add2(v[r][c][i], res[i]);
+                        const uint4 stored = to_raw<T>(v[r][c]);
+                        *reinterpret_cast<uint4*>(sum + e) = stored;
+                        to_pairs<T>(v[r][c], stored);                // the norm is of the stored value
                     }
-#pragma unroll
-                    for (int i = 0; i < NP; ++i) acc = add2(acc, v[i]);
                 }
-                keep_packed(xp[r][c]);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) acc = add2(acc, v[r][c][i]);
             }
             mean[r] = halves_sum(acc);
         }
         lanes_sum<R>(mean, ra.lanes);
         if constexpr (R == 1) {
-            if (ra.warps_per_row > 1) warps_sum<1>(mean, ra.warps_per_row, warp_in_row, group, red);
+            if (ra.warps_per_row > 1) warps_sum<1>(mean, ra.warps_per_row, warp_in_row, group + 1, red);
         }
         // Every warp of the row has lifted its part of the stage (one warp: its lanes meet here).
         __syncwarp();
-        if (leader) ring.fill(ring.stage, x, second, row0 + ring.stages * step, ra.step_rows, rows, hidden);
+        if (leader) ring.fill(ring.stage, x, second, none, row0 + ring.stages * step, ra.step_rows, rows, hidden);
         ring.next();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            mean[r] *= -inv_hidden;
-            const Pair shift = pair(mean[r]);
+            const Pair shift = pair(-mean[r] * inv_hidden);
             Pair acc = 0;
 #pragma unroll
             for (int c = 0; c < CPT; ++c) {
-                if (vec0 + c * vec_step < ra.vectors) {
-                    Pair v[NP];
-                    to_pairs<T>(v, xp[r][c]);
+                if (FULL || vec0 + c * 32 < ra.vectors) {
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
-                        v[i] = add2(v[i], shift);
-                        acc = fma2(v[i], v[i], acc);
+                        v[r][c][i] = add2(v[r][c][i], shift);
+                        acc = fma2(v[r][c][i], v[r][c][i], acc);
                     }
                 }
-                keep_packed(xp[r][c]);
             }
             rstd[r] = halves_sum(acc);
         }
         lanes_sum<R>(rstd, ra.lanes);
         if constexpr (R == 1) {
-            if (ra.warps_per_row > 1) warps_sum<1>(rstd, ra.warps_per_row, warp_in_row, group, red + 16);
+            if (ra.warps_per_row > 1) warps_sum<1>(rstd, ra.warps_per_row, warp_in_row, group + 1, red + 16);
         }
 #pragma unroll
         for (int r = 0; r < R; ++r) rstd[r] = rsqrtf(fmaf(rstd[r], inv_hidden, epsilon));
+        T* out = y + e0;
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
-            const int vec = vec0 + c * vec_step;
-            if (vec < ra.vectors) {
+            if (FULL || vec0 + c * 32 < ra.vectors) {
                 Pair wv[NP], bv[NP];
-                read_pairs<NP>(wv, ws + vec * VEC);
-                read_pairs<NP>(bv, bs + vec * VEC);
+                read_pairs<NP>(wv, ws, vec0 + c * 32, ra.vectors);
+                read_pairs<NP>(bv, bs, vec0 + c * 32, ra.vectors);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const int in_step = r * per_warp + lane_row;
-                    if (row0 + in_step < rows) {
-                        const Pair shift = pair(mean[r]), scale = pair(rstd[r]);
-                        Pair v[NP];
-                        to_pairs<T>(v, xp[r][c]);
+                    if (R == 1 || r * per_warp + lane_row < left) {
+                        const Pair scale = pair(rstd[r]);
 #pragma unroll
-                        for (int i = 0; i < NP; ++i) v[i] = fma2(mul2(add2(v[i], shift), scale), wv[i], bv[i]);
-                        *reinterpret_cast<uint4*>(y + (row0 + in_step) * hidden + vec * VEC) = to_raw<T>(v);
+                        for (int i = 0; i < NP; ++i) v[r][c][i] = fma2(mul2(v[r][c][i], scale), wv[i], bv[i]);
+                        *reinterpret_cast<uint4*>(out + r * per_warp * hidden + c * (32 * VEC)) = to_raw<T>(v[r][c]);
                     }
                 }
             }
@@ -349,25 +344,27 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
     }
 }
 
-// CPT: vectors per lane in the row phase. COLS: vectors per thread and row in the column phase. partial: [gridDim.x][2][hidden].
-template <typename T, int CPT, int COLS, bool FUSED>
+// CPT: vectors per lane in the row phase (FULL: exactly the row's). COLS: vectors per thread and row in the column phase.
+// partial: [gridDim.x][2][hidden].
+template <typename T, int CPT, int COLS, bool FULL, bool FUSED>
 __global__ void __launch_bounds__(kBackwardThreads, 1)
 layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const T* __restrict__ dy, const T* __restrict__ x,
                                const T* __restrict__ w, const T* residual, long long rows, int hidden, float epsilon, const RingArgs ra,
                                const DropoutArgs args) {
-    constexpr int VEC = 16 / sizeof(T), NP = VEC / 2, R = kLaneVectors / CPT, RC = kLaneVectors / COLS;
+    constexpr int VEC = 16 / sizeof(T), NP = VEC / 2, R = rows_at_once(CPT), RC = kTileVectors / COLS;
     extern __shared__ __align__(128) unsigned char shared[];
-    __shared__ float4 stats[2][kMaxTileRows];                // -mean, rstd, -c1, -c2 of the tile's rows
+    __shared__ ulonglong2 stats[2][kMaxTileRows][2];         // -mean, rstd; -c1, -c2 of the tile's rows, each as a pair of equals
     float* ws = reinterpret_cast<float*>(shared + kVectorsOffset);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int unit = warp / ra.warps_per_row, warp_in_row = warp - unit * ra.warps_per_row;
     const int units = (blockDim.x >> 5) / ra.warps_per_row;
     const int per_warp = 32 / ra.lanes;
-    const int lane_row = lane / ra.lanes, vec0 = warp_in_row * 32 + (lane & (ra.lanes - 1)), vec_step = ra.warps_per_row * ra.lanes;
+    const int lane_row = lane / ra.lanes, vec0 = warp_in_row * (32 * CPT) + (lane & (ra.lanes - 1));
     float* red = reinterpret_cast<float*>(shared + kSumsOffset) + unit * 64;
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
     const long long step = static_cast<long long>(gridDim.x) * ra.step_rows;
     const long long first = static_cast<long long>(blockIdx.x) * ra.step_rows;
+    const T* none = nullptr;
     Ring ring{};
     ring.row_bytes = static_cast<unsigned>(hidden) * sizeof(T);
     ring.tensor_bytes = ra.step_rows * ring.row_bytes;
@@ -378,7 +375,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     ring.status = ra.status;
     if (threadIdx.x == 0) {
         ring.init();
-        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, dy, first + s * step, ra.step_rows, rows, hidden);
+        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, dy, none, first + s * step, ra.step_rows, rows, hidden);
     }
     stage_vector(ws, w, ra.vectors);
     const Philox gen(args);
@@ -386,54 +383,54 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     const int row_group = COLS == 1 ? threadIdx.x / ra.vectors : 0;
     const int column = COLS == 1 ? threadIdx.x - row_group * ra.vectors : threadIdx.x;      // in vectors
     const bool works = COLS > 1 || row_group < ra.groups;
+    const unsigned column_bytes = row_group * ring.row_bytes + column * 16, next_rows = ra.groups * ring.row_bytes;
+    const unsigned lane_bytes = lane_row * ring.row_bytes + vec0 * 16, next_row = per_warp * ring.row_bytes;
+    const int next_elements = ra.groups * hidden;
     __syncthreads();
     Pair wv[COLS][NP], aw[COLS][NP], ab[COLS][NP];
 #pragma unroll
     for (int c = 0; c < COLS; ++c) {
         const int vec = column + c * blockDim.x;
-        if (vec < ra.vectors) read_pairs<NP>(wv[c], ws + vec * VEC);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            if (vec >= ra.vectors) wv[c][i] = 0;
-            aw[c][i] = 0;
-            ab[c][i] = 0;
-        }
+        for (int i = 0; i < NP; ++i) wv[c][i] = aw[c][i] = ab[c][i] = 0;
+        if (vec < ra.vectors) read_pairs<NP>(wv[c], ws, vec, ra.vectors);
     }
 
     int buffer = 0;
     for (long long row0 = first; row0 < rows; row0 += step, buffer ^= 1) {
         const int tile_rows = rows - row0 < ra.step_rows ? static_cast<int>(rows - row0) : ra.step_rows;
+        const long long e0 = (row0 + row_group) * hidden + column * VEC;       // the thread's first element in the column phase
         // The residual is needed last: on its way past the ring while the row sums are taken.
         uint4 rp[RC][COLS];
+        if (residual != nullptr && works) {
 #pragma unroll
-        for (int k = 0; k < RC; ++k)
+            for (int k = 0; k < RC; ++k)
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                const int row = k * ra.groups + row_group, vec = column + c * blockDim.x;
-                rp[k][c] = residual != nullptr && works && row < tile_rows && vec < ra.vectors
-                               ? __ldcs(reinterpret_cast<const uint4*>(residual + (row0 + row) * hidden + vec * VEC)) : make_uint4(0u, 0u, 0u, 0u);
-            }
+                for (int c = 0; c < COLS; ++c)
+                    if (k * ra.groups + row_group < tile_rows && (COLS == 1 || column + c * blockDim.x < ra.vectors))
+                        rp[k][c] = __ldcs(reinterpret_cast<const uint4*>(residual + e0 + k * next_elements + c * blockDim.x * VEC));
+        }
         const unsigned char* stage = ring.wait();
         // ---- rows: four sums each
         for (int base = unit * R * per_warp; base < tile_rows; base += units * R * per_warp) {
-            uint4 xp[R][CPT], gp[R][CPT];
+            const unsigned char* at = stage + base * ring.row_bytes + lane_bytes;
+            Pair v[R][CPT][NP];
+            uint4 gp[R][CPT];
             float mean[R], sums[3 * R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const int row = base + r * per_warp + lane_row;
                 Pair acc = 0;
 #pragma unroll
                 for (int c = 0; c < CPT; ++c) {
-                    const int vec = vec0 + c * vec_step;
-                    const unsigned char* at = stage + row * ring.row_bytes + vec * 16;
-                    const bool in = row < tile_rows && vec < ra.vectors;
-                    xp[r][c] = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
-                    gp[r][c] = in ? *reinterpret_cast<const uint4*>(at + ring.tensor_bytes) : make_uint4(0u, 0u, 0u, 0u);
-                    Pair v[NP];
-                    to_pairs<T>(v, xp[r][c]);
+                    gp[r][c] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) acc = add2(acc, v[i]);
-                    keep_packed(xp[r][c]);
+                    for (int i = 0; i < NP; ++i) v[r][c][i] = 0;
+                    if ((R == 1 || base + r * per_warp + lane_row < tile_rows) && (FULL || vec0 + c * 32 < ra.vectors)) {
+                        gp[r][c] = *reinterpret_cast<const uint4*>(at + ring.tensor_bytes + r * next_row + c * 512);
+                        to_pairs<T>(v[r][c], *reinterpret_cast<const uint4*>(at + r * next_row + c * 512));
+                    }
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) acc = add2(acc, v[r][c][i]);
                 }
                 mean[r] = halves_sum(acc);
             }
@@ -449,19 +446,17 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
             }
 #pragma unroll
             for (int c = 0; c < CPT; ++c) {
-                const int vec = vec0 + c * vec_step;
-                if (vec < ra.vectors) {
+                if (FULL || vec0 + c * 32 < ra.vectors) {
                     Pair wr[NP];
-                    read_pairs<NP>(wr, ws + vec * VEC);
+                    read_pairs<NP>(wr, ws, vec0 + c * 32, ra.vectors);
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
                         const Pair shift = pair(mean[r]);
-                        Pair v[NP], g[NP];
-                        to_pairs<T>(v, xp[r][c]);
+                        Pair g[NP];
                         to_pairs<T>(g, gp[r][c]);
 #pragma unroll
                         for (int i = 0; i < NP; ++i) {
-                            const Pair d = add2(v[i], shift), gw = mul2(g[i], wr[i]);
+                            const Pair d = add2(v[r][c][i], shift), gw = mul2(g[i], wr[i]);
                             s0[r] = fma2(d, d, s0[r]);
                             s1[r] = add2(s1[r], gw);
                             s2[r] = fma2(gw, d, s2[r]);
@@ -484,36 +479,40 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
                 for (int r = 0; r < R; ++r) {
                     const int row = base + r * per_warp + lane_row;
                     const float rstd = rsqrtf(fmaf(sums[r], inv_hidden, epsilon));
-                    if (row < tile_rows) stats[buffer][row] = make_float4(mean[r], rstd, -sums[R + r] * inv_hidden, -(sums[2 * R + r] * inv_hidden * rstd));
+                    if (row < tile_rows) {
+                        stats[buffer][row][0] = make_ulonglong2(pair(mean[r]), pair(rstd));
+                        stats[buffer][row][1] = make_ulonglong2(pair(-sums[R + r] * inv_hidden), pair(-(sums[2 * R + r] * inv_hidden * rstd)));
+                    }
                 }
             }
         }
         __syncthreads();
         // Every thread is past the columns of the tile before: its stage is free.
         if (threadIdx.x == 0 && row0 != first)
-            ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, row0 + (ring.stages - 1) * step, ra.step_rows, rows, hidden);
+            ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, none, row0 + (ring.stages - 1) * step, ra.step_rows, rows, hidden);
         // ---- columns
         if (works) {
+            const unsigned char* at = stage + column_bytes;
 #pragma unroll
             for (int k = 0; k < RC; ++k) {
                 const int row = k * ra.groups + row_group;
                 if (row < tile_rows) {
-                    const float4 st = stats[buffer][row];
-                    const Pair shift = pair(st.x), rstd = pair(st.y), c1 = pair(st.z), c2 = pair(st.w);
+                    const ulonglong2 st = stats[buffer][row][0], cs = stats[buffer][row][1];
 #pragma unroll
                     for (int c = 0; c < COLS; ++c) {
-                        const int vec = column + c * blockDim.x;
-                        if (vec < ra.vectors) {
-                            const unsigned char* at = stage + row * ring.row_bytes + vec * 16;
-                            const long long e = (row0 + row) * hidden + vec * VEC;
+                        if (COLS == 1 || column + c * blockDim.x < ra.vectors) {
+                            const unsigned char* here = at + k * next_rows + c * blockDim.x * 16;
+                            const long long e = e0 + k * next_elements + c * blockDim.x * VEC;
                             Pair v[NP], g[NP], out[NP];
-                            to_pairs<T>(v, *reinterpret_cast<const uint4*>(at));
-                            to_pairs<T>(g, *reinterpret_cast<const uint4*>(at + ring.tensor_bytes));
-                            to_pairs<T>(out, rp[k][c]);
+                            to_pairs<T>(v, *reinterpret_cast<const uint4*>(here));
+                            to_pairs<T>(g, *reinterpret_cast<const uint4*>(here + ring.tensor_bytes));
+#pragma unroll
+                            for (int i = 0; i < NP; ++i) out[i] = 0;
+                            if (residual != nullptr) to_pairs<T>(out, rp[k][c]);
 #pragma unroll
                             for (int i = 0; i < NP; ++i) {
-                                const Pair xh = mul2(add2(v[i], shift), rstd);
-                                out[i] = fma2(rstd, fma2(xh, c2, fma2(g[i], wv[c][i], c1)), out[i]);
+                                const Pair xh = mul2(add2(v[i], st.x), st.y);
+                                out[i] = fma2(st.y, fma2(xh, cs.y, fma2(g[i], wv[c][i], cs.x)), out[i]);
                                 aw[c][i] = fma2(g[i], xh, aw[c][i]);
                                 ab[c][i] = add2(ab[c][i], g[i]);
                             }
@@ -533,7 +532,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     // One partial row of dw and of db per CTA: its row groups add up one after the other, in the memory of the ring, whose copies
     // have all been waited for.
     float* out_w = partial + static_cast<long long>(blockIdx.x) * 2 * hidden;
-    float* joined = reinterpret_cast<float*>(shared + ra.data_offset);
+    Pair* joined = reinterpret_cast<Pair*>(shared + ra.data_offset);           // [pair][dw, db][vector]: no bank conflicts
     const int groups = COLS == 1 ? ra.groups : 1;
     for (int k = 0; k < groups; ++k) {
         __syncthreads();
@@ -544,16 +543,15 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
                 if (vec < ra.vectors) {
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
-                        const int at = (i * 2) * ra.vectors + vec;       // pairs, one per thread: no bank conflicts
-                        Pair* s = reinterpret_cast<Pair*>(joined);
+                        const int at = (i * 2) * ra.vectors + vec;
                         Pair tw = aw[c][i], tb = ab[c][i];
                         if (k > 0) {
-                            tw = add2(s[at], tw);
-                            tb = add2(s[at + ra.vectors], tb);
+                            tw = add2(joined[at], tw);
+                            tb = add2(joined[at + ra.vectors], tb);
                         }
                         if (k + 1 < groups) {
-                            s[at] = tw;
-                            s[at + ra.vectors] = tb;
+                            joined[at] = tw;
+                            joined[at + ra.vectors] = tb;
                         } else {
                             *reinterpret_cast<Pair*>(out_w + vec * VEC + 2 * i) = tw;
                             *reinterpret_cast<Pair*>(out_w + hidden + vec * VEC + 2 * i) = tb;

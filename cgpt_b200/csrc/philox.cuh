@@ -54,20 +54,17 @@ struct Philox {
     }
 };
 
-// One element's decision on 16 bits. The product is rounded by itself (no contraction with a residual added to it), so that every
-// kernel gives the same bits for the same element.
+// One element's decision on the high half of `u` (its low half may hold anything: u >= t * 2^16 exactly if its high half >= t).
+// The product is rounded by itself (no contraction with a residual added to it), so that every kernel gives the same bits.
 __device__ __forceinline__ float decide(float v, std::uint32_t u, std::uint32_t threshold, float scale) {
-    return u >= threshold ? __fmul_rn(v, scale) : 0.f;
+    return u >= threshold << 16 ? __fmul_rn(v, scale) : 0.f;
 }
 
 // Applies a block's eight decisions to eight consecutive elements. Dropped elements become +0 whatever they held.
 __device__ __forceinline__ void apply_block(float (&v)[8], const uint4& bits, std::uint32_t threshold, float scale) {
     const std::uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const std::uint32_t u = (i & 1) != 0 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-        v[i] = decide(v[i], u, threshold, scale);
-    }
+    for (int i = 0; i < 8; ++i) v[i] = decide(v[i], (i & 1) != 0 ? w[i >> 1] : w[i >> 1] << 16, threshold, scale);
 }
 
 // The decision of one element, for places that cannot share a block (its other seven decisions are thrown away).
@@ -75,8 +72,7 @@ __device__ __forceinline__ float apply_one(float v, const Philox& gen, long long
     const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
     const int i = static_cast<int>(e & 7);
     const std::uint32_t w = i < 4 ? (i < 2 ? c.x : c.y) : (i < 6 ? c.z : c.w);
-    const std::uint32_t u = (i & 1) != 0 ? w >> 16 : w & 0xffffu;
-    return decide(v, u, a.threshold, a.scale);
+    return decide(v, (i & 1) != 0 ? w : w << 16, a.threshold, a.scale);
 }
 
 // The dropout map of VEC elements that start at element e of the tensor (e % VEC == 0 for VEC > 1).
@@ -88,10 +84,10 @@ __device__ __forceinline__ void drop_vec(float (&v)[VEC], const Philox& gen, lon
         const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
         const bool high = (e & 4) != 0;
         const std::uint32_t w0 = high ? c.z : c.x, w1 = high ? c.w : c.y;
-        v[0] = decide(v[0], w0 & 0xffffu, args.threshold, args.scale);
-        v[1] = decide(v[1], w0 >> 16, args.threshold, args.scale);
-        v[2] = decide(v[2], w1 & 0xffffu, args.threshold, args.scale);
-        v[3] = decide(v[3], w1 >> 16, args.threshold, args.scale);
+        v[0] = decide(v[0], w0 << 16, args.threshold, args.scale);
+        v[1] = decide(v[1], w0, args.threshold, args.scale);
+        v[2] = decide(v[2], w1 << 16, args.threshold, args.scale);
+        v[3] = decide(v[3], w1, args.threshold, args.scale);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = apply_one(v[i], gen, e + i, args);
