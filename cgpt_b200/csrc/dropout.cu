@@ -11,40 +11,72 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Eight consecutive elements per thread and trip: one generator block. VECTOR: 16-byte accesses (aligned bases).
-template <typename T, bool VECTOR>
+// Aligned tensors: BLOCKS generator blocks of eight elements per thread and trip, all loads of a trip (the residual's too) on
+// their way before the first block is worked out: four 16-byte loads a thread.
+template <typename T, bool RESIDUAL>
+__global__ void __launch_bounds__(kThreads)
+dropout_vector_kernel(T* out, const T* in, const T* residual, long long count, const DropoutArgs args) {
+    constexpr int V = 16 / sizeof(T), N = 8 / V;              // 16-byte vectors per block
+    constexpr int BLOCKS = 4 / (N * (RESIDUAL ? 2 : 1));
+    const PhiloxOf<!RESIDUAL> gen(args);   // round keys kept: 28.7 -> 26.8 us at 32768 x 1024 f16, but 67.3 -> 69.5 with a residual (32768 x 2048)
+    const long long whole = count >> 3;
+    if (blockIdx.x == 0 && threadIdx.x < (count & 7)) {       // the last elements fill no block
+        const long long e = whole * 8 + threadIdx.x;
+        float v = to_f32<T>(in[e]);
+        if (args.threshold != 0) v = apply_one(v, gen, e, args);
+        out[e] = from_f32<T>(RESIDUAL ? v + to_f32<T>(residual[e]) : v);
+    }
+    const long long stride = static_cast<long long>(gridDim.x) * kThreads;
+    for (long long block0 = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; block0 < whole; block0 += stride * BLOCKS) {
+        uint4 x[BLOCKS][N], r[BLOCKS][N];
+#pragma unroll
+        for (int k = 0; k < BLOCKS; ++k) {
+            const long long block = block0 + k * stride;
+            if (block < whole) {
+#pragma unroll
+                for (int c = 0; c < N; ++c) {
+                    x[k][c] = __ldcs(reinterpret_cast<const uint4*>(in) + block * N + c);
+                    if constexpr (RESIDUAL) r[k][c] = __ldcs(reinterpret_cast<const uint4*>(residual) + block * N + c);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < BLOCKS; ++k) {
+            const long long block = block0 + k * stride;
+            if (block < whole) {
+                float v[8];
+#pragma unroll
+                for (int c = 0; c < N; ++c) unpack_pack(*reinterpret_cast<float(*)[V]>(&v[c * V]), *reinterpret_cast<const Pack<T, V>*>(&x[k][c]));
+                if (args.threshold != 0) apply_block(v, gen.block(static_cast<std::uint32_t>(block)), args.threshold, args.scale);
+#pragma unroll
+                for (int c = 0; c < N; ++c) {
+                    if constexpr (RESIDUAL) {
+                        float res[V];
+                        unpack_pack(res, *reinterpret_cast<const Pack<T, V>*>(&r[k][c]));
+#pragma unroll
+                        for (int i = 0; i < V; ++i) v[c * V + i] += res[i];
+                    }
+                    store_vec<T, V>(out + block * 8 + c * V, *reinterpret_cast<const float(*)[V]>(&v[c * V]));
+                }
+            }
+        }
+    }
+}
+
+// Any alignment, element by element; a thread still has the eight elements of a block.
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
 dropout_kernel(T* out, const T* in, const T* residual, long long count, const DropoutArgs args) {
     const Philox gen(args);
     const long long stride = static_cast<long long>(gridDim.x) * kThreads * 8;
     for (long long i = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) * 8; i < count; i += stride) {
         float v[8];
-        const bool whole = VECTOR && i + 8 <= count;
-        if (whole) {
-            constexpr int V = 16 / sizeof(T);
 #pragma unroll
-            for (int c = 0; c < 8; c += V) load_vec_stream<T, V>(*reinterpret_cast<float(*)[V]>(&v[c]), in + i + c);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = i + k < count ? to_f32<T>(in[i + k]) : 0.f;
-        }
+        for (int k = 0; k < 8; ++k) v[k] = i + k < count ? to_f32<T>(in[i + k]) : 0.f;
         if (args.threshold != 0) apply_block(v, gen.block(static_cast<std::uint32_t>(i >> 3)), args.threshold, args.scale);
-        if (whole) {
-            constexpr int V = 16 / sizeof(T);
-            if (residual != nullptr) {
-                float r[8];
 #pragma unroll
-                for (int c = 0; c < 8; c += V) load_vec_stream<T, V>(*reinterpret_cast<float(*)[V]>(&r[c]), residual + i + c);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] += r[k];
-            }
-#pragma unroll
-            for (int c = 0; c < 8; c += V) store_vec<T, V>(out + i + c, *reinterpret_cast<float(*)[V]>(&v[c]));
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (i + k < count) out[i + k] = from_f32<T>(residual != nullptr ? v[k] + to_f32<T>(residual[i + k]) : v[k]);
-        }
+        for (int k = 0; k < 8; ++k)
+            if (i + k < count) out[i + k] = from_f32<T>(residual != nullptr ? v[k] + to_f32<T>(residual[i + k]) : v[k]);
     }
 }
 
@@ -61,9 +93,10 @@ int run(void* out, const void* in, const void* residual, std::size_t count, floa
     auto s = static_cast<cudaStream_t>(stream);
     const bool al = aligned16(out) && aligned16(in) && aligned16(residual);
     CGPT_DISPATCH_DTYPE(dtype, T, {
-        auto kernel = al ? dropout_kernel<T, true> : dropout_kernel<T, false>;
-        const std::size_t need = (count + kThreads * 8 - 1) / (kThreads * 8);
-        const std::size_t cap = static_cast<std::size_t>(kNumSMs) * resident_ctas_per_sm(reinterpret_cast<const void*>(kernel), kThreads, 0);
+        auto kernel = !al ? dropout_kernel<T> : residual != nullptr ? dropout_vector_kernel<T, true> : dropout_vector_kernel<T, false>;
+        const std::size_t per_thread = !al ? 8 : residual != nullptr ? 32 / sizeof(T) : 64 / sizeof(T);   // elements per trip
+        const std::size_t need = (count + kThreads * per_thread - 1) / (kThreads * per_thread);
+        constexpr std::size_t cap = std::size_t{1} << 30;
         kernel<<<static_cast<unsigned>(need < cap ? need : cap), kThreads, 0, s>>>(
             static_cast<T*>(out), static_cast<const T*>(in), static_cast<const T*>(residual), static_cast<long long>(count), args);
         count_launch();

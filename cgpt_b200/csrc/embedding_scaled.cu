@@ -33,28 +33,43 @@ constexpr int kMaxDigitBits = 9;
 constexpr int kClusterThreads = 1024;
 constexpr int kMaxCluster = 16;
 
+// kLookups consecutive tokens per group of threads and trip: their ids, then their rows, are loaded together, and the decisions
+// (about 10 instructions an element, most of the kernel's work) are made while the rows are on their way.
+constexpr int kLookups = 4;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
 scaled_embedding_forward_kernel(T* __restrict__ out, const std::uint32_t* __restrict__ ids, const T* __restrict__ weight,
-                                long long tokens, std::uint32_t vocab, long long hidden, float scale, int group,
-                                const DropoutArgs args) {
-    const Philox gen(args);
+                                long long tokens, std::uint32_t vocab, int hidden, float scale, int group, const DropoutArgs args) {
+    using Raw = typename RawVec<sizeof(T) * VEC>::type;
+    const HoistedPhilox gen(args);
     const int lane = threadIdx.x % group;
-    const long long groups = static_cast<long long>(gridDim.x) * (kThreads / group);
-    for (long long t = static_cast<long long>(blockIdx.x) * (kThreads / group) + threadIdx.x / group; t < tokens; t += groups) {
-        const std::uint32_t id = ids[t];
-        for (long long c = static_cast<long long>(lane) * VEC; c < hidden; c += static_cast<long long>(group) * VEC) {
-            float v[VEC];
-            if (id < vocab) {
-                load_vec<T, VEC>(v, weight + static_cast<long long>(id) * hidden + c);
+    const long long step = static_cast<long long>(gridDim.x) * (kThreads / group) * kLookups;
+    for (long long t0 = (static_cast<long long>(blockIdx.x) * (kThreads / group) + threadIdx.x / group) * kLookups; t0 < tokens; t0 += step) {
+        std::uint32_t id[kLookups];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[i] *= scale;
-                if (args.threshold != 0) drop_vec<VEC>(v, gen, t * hidden + c, args);
-            } else {
+        for (int k = 0; k < kLookups; ++k) id[k] = t0 + k < tokens ? ids[t0 + k] : 0xffffffffu;
+        for (int c = lane * VEC; c < hidden; c += group * VEC) {
+            Pack<T, VEC> row[kLookups];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+            for (int k = 0; k < kLookups; ++k)
+                if (id[k] < vocab) *reinterpret_cast<Raw*>(&row[k]) = *reinterpret_cast<const Raw*>(weight + static_cast<long long>(id[k]) * hidden + c);
+#pragma unroll
+            for (int k = 0; k < kLookups; ++k) {
+                if (t0 + k < tokens) {
+                    const long long e = (t0 + k) * hidden + c;
+                    float v[VEC];
+                    if (id[k] < vocab) {
+                        unpack_pack(v, row[k]);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) v[i] *= scale;
+                        if (args.threshold != 0) drop_vec<VEC>(v, gen, e, args);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+                    }
+                    store_vec<T, VEC>(out + e, v);
+                }
             }
-            store_vec<T, VEC>(out + t * hidden + c, v);
         }
     }
 }
@@ -387,7 +402,7 @@ scaled_embedding_sum_kernel(T* dw, const T* __restrict__ dout, const GradArgs g,
         }
         return;
     }
-    const Philox gen(args);
+    const HoistedPhilox gen(args);
     // The CTA's tokens, with one id before and one behind them; no neighbour: an id that no token has (vocab marks skipped ones).
     const int span = g.groups * kChunk;
     const long long lo = static_cast<long long>(blockIdx.x) * span;
@@ -656,11 +671,10 @@ extern "C" int cgpt_scaled_embedding_forward(void* out, const uint32_t* ids, con
         const bool vector = hidden % V == 0 && aligned16(out) && aligned16(weight);
         auto kernel = vector ? scaled_embedding_forward_kernel<T, V> : scaled_embedding_forward_kernel<T, 1>;
         const int group = group_for(hidden, vector ? V : 1);
-        const std::size_t per_cta = kThreads / group, need = (tokens + per_cta - 1) / per_cta;
-        const std::size_t cap = static_cast<std::size_t>(kNumSMs) * resident_ctas_per_sm(reinterpret_cast<const void*>(kernel), kThreads, 0);
-        kernel<<<static_cast<unsigned>(need < cap ? need : cap), kThreads, 0, s>>>(
+        const std::size_t per_cta = static_cast<std::size_t>(kThreads / group) * kLookups, need = (tokens + per_cta - 1) / per_cta;
+        kernel<<<static_cast<unsigned>(need), kThreads, 0, s>>>(
             static_cast<T*>(out), ids, static_cast<const T*>(weight), static_cast<long long>(tokens), static_cast<std::uint32_t>(vocab),
-            static_cast<long long>(hidden), scale, group, args);
+            static_cast<int>(hidden), scale, group, args);
         count_launch();
         CGPT_LAUNCH_CHECK();
     });

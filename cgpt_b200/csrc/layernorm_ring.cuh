@@ -102,8 +102,8 @@ __device__ __forceinline__ uint4 to_raw(const Pair (&p)[8 / sizeof(T)]) {
         return make_uint4(two_of<T>(p[0]), two_of<T>(p[1]), two_of<T>(p[2]), two_of<T>(p[3]));
     }
 }
-template <typename T>
-__device__ __forceinline__ void drop_pairs(Pair (&p)[8 / sizeof(T)], const Philox& gen, long long e, const DropoutArgs& args) {
+template <typename T, typename Generator>
+__device__ __forceinline__ void drop_pairs(Pair (&p)[8 / sizeof(T)], const Generator& gen, long long e, const DropoutArgs& args) {
     constexpr int VEC = 16 / sizeof(T);
     float v[VEC];
 #pragma unroll
@@ -378,7 +378,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
         for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, dy, none, first + s * step, ra.step_rows, rows, hidden);
     }
     stage_vector(ws, w, ra.vectors);
-    const Philox gen(args);
+    const HoistedPhilox gen(args);
     // Column phase: with COLS == 1 the threads cover `groups` rows at a time, vector after vector, row after row.
     const int row_group = COLS == 1 ? threadIdx.x / ra.vectors : 0;
     const int column = COLS == 1 ? threadIdx.x - row_group * ra.vectors : threadIdx.x;      // in vectors

@@ -26,33 +26,51 @@ struct DropoutArgs {
     float scale;                       // 65536 / (65536 - threshold)
 };
 
-// The generator of one call with seed, step and site in registers.
-struct Philox {
-    std::uint32_t k0, k1, site, step_lo, step_hi;
+// The generator of one call with seed, step and site in registers. HOIST: the round keys too (20 registers), which saves a third
+// of a block's instructions besides its products where registers are free.
+template <bool HOIST>
+struct PhiloxOf {
+    std::uint32_t k0[HOIST ? 10 : 1], k1[HOIST ? 10 : 1], site, step_lo, step_hi;
 
-    __device__ __forceinline__ explicit Philox(const DropoutArgs& a) {
+    __device__ __forceinline__ explicit PhiloxOf(const DropoutArgs& a) {
         const unsigned long long seed = a.threshold != 0 ? a.state[0] : 0ull, step = a.threshold != 0 ? a.state[1] : 0ull;
-        k0 = static_cast<std::uint32_t>(seed);
-        k1 = static_cast<std::uint32_t>(seed >> 32);
+        k0[0] = static_cast<std::uint32_t>(seed);
+        k1[0] = static_cast<std::uint32_t>(seed >> 32);
+        if constexpr (HOIST) {
+#pragma unroll
+            for (int r = 1; r < 10; ++r) {
+                k0[r] = k0[r - 1] + 0x9E3779B9u;
+                k1[r] = k1[r - 1] + 0xBB67AE85u;
+                asm volatile("" : "+r"(k0[r]), "+r"(k1[r]));   // or they are added up again at every use
+            }
+        }
         step_lo = static_cast<std::uint32_t>(step);
         step_hi = static_cast<std::uint32_t>(step >> 32);
         site = a.site;
     }
     __device__ __forceinline__ uint4 block(std::uint32_t index) const {
         uint4 c = make_uint4(index, site, step_lo, step_hi);
-        std::uint32_t ka = k0, kb = k1;
+        std::uint32_t ka = k0[0], kb = k1[0];
 #pragma unroll
         for (int r = 0; r < 10; ++r) {
+            if constexpr (HOIST) {
+                ka = k0[r];
+                kb = k1[r];
+            }
             const unsigned long long p = static_cast<unsigned long long>(0xD2511F53u) * c.x;
             const unsigned long long q = static_cast<unsigned long long>(0xCD9E8D57u) * c.z;
             c = make_uint4(static_cast<std::uint32_t>(q >> 32) ^ c.y ^ ka, static_cast<std::uint32_t>(q),
                            static_cast<std::uint32_t>(p >> 32) ^ c.w ^ kb, static_cast<std::uint32_t>(p));
-            ka += 0x9E3779B9u;
-            kb += 0xBB67AE85u;
+            if constexpr (!HOIST) {
+                ka += 0x9E3779B9u;
+                kb += 0xBB67AE85u;
+            }
         }
         return c;
     }
 };
+using Philox = PhiloxOf<false>;
+using HoistedPhilox = PhiloxOf<true>;
 
 // One element's decision on the high half of `u` (its low half may hold anything: u >= t * 2^16 exactly if its high half >= t).
 // The product is rounded by itself (no contraction with a residual added to it), so that every kernel gives the same bits.
@@ -68,7 +86,8 @@ __device__ __forceinline__ void apply_block(float (&v)[8], const uint4& bits, st
 }
 
 // The decision of one element, for places that cannot share a block (its other seven decisions are thrown away).
-__device__ __forceinline__ float apply_one(float v, const Philox& gen, long long e, const DropoutArgs& a) {
+template <typename Generator>
+__device__ __forceinline__ float apply_one(float v, const Generator& gen, long long e, const DropoutArgs& a) {
     const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
     const int i = static_cast<int>(e & 7);
     const std::uint32_t w = i < 4 ? (i < 2 ? c.x : c.y) : (i < 6 ? c.z : c.w);
@@ -76,8 +95,8 @@ __device__ __forceinline__ float apply_one(float v, const Philox& gen, long long
 }
 
 // The dropout map of VEC elements that start at element e of the tensor (e % VEC == 0 for VEC > 1).
-template <int VEC>
-__device__ __forceinline__ void drop_vec(float (&v)[VEC], const Philox& gen, long long e, const DropoutArgs& args) {
+template <int VEC, typename Generator>
+__device__ __forceinline__ void drop_vec(float (&v)[VEC], const Generator& gen, long long e, const DropoutArgs& args) {
     if constexpr (VEC == 8) {
         apply_block(v, gen.block(static_cast<std::uint32_t>(e >> 3)), args.threshold, args.scale);
     } else if constexpr (VEC == 4) {
