@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(kThreads)
 dropout_vector_kernel(T* out, const T* in, const T* residual, long long count, const DropoutArgs args) {
     constexpr int V = 16 / sizeof(T), N = 8 / V;              // 16-byte vectors per block
     constexpr int BLOCKS = 4 / (N * (RESIDUAL ? 2 : 1));
-    const PhiloxOf<!RESIDUAL> gen(args);   // round keys kept: 28.7 -> 26.8 us at 32768 x 1024 f16, but 67.3 -> 69.5 with a residual (32768 x 2048)
+    const PhiloxOf<!RESIDUAL> gen(args);   // round keys kept only where nothing else is on its way
     const long long whole = count >> 3;
     if (blockIdx.x == 0 && threadIdx.x < (count & 7)) {       // the last elements fill no block
         const long long e = whole * 8 + threadIdx.x;
@@ -27,37 +27,41 @@ dropout_vector_kernel(T* out, const T* in, const T* residual, long long count, c
         out[e] = from_f32<T>(RESIDUAL ? v + to_f32<T>(residual[e]) : v);
     }
     const long long stride = static_cast<long long>(gridDim.x) * kThreads;
-    for (long long block0 = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; block0 < whole; block0 += stride * BLOCKS) {
-        uint4 x[BLOCKS][N], r[BLOCKS][N];
+    uint4 x[BLOCKS][N], r[BLOCKS][N];
+    auto load = [&](int k, long long block) {
 #pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            const long long block = block0 + k * stride;
-            if (block < whole) {
-#pragma unroll
-                for (int c = 0; c < N; ++c) {
-                    x[k][c] = __ldcs(reinterpret_cast<const uint4*>(in) + block * N + c);
-                    if constexpr (RESIDUAL) r[k][c] = __ldcs(reinterpret_cast<const uint4*>(residual) + block * N + c);
-                }
-            }
+        for (int c = 0; c < N; ++c) {
+            x[k][c] = __ldcs(reinterpret_cast<const uint4*>(in) + block * N + c);
+            if constexpr (RESIDUAL) r[k][c] = __ldcs(reinterpret_cast<const uint4*>(residual) + block * N + c);
         }
+    };
+    auto finish = [&](int k, long long block) {
+        Pair v[4];
 #pragma unroll
-        for (int k = 0; k < BLOCKS; ++k) {
-            const long long block = block0 + k * stride;
-            if (block < whole) {
-                float v[8];
+        for (int c = 0; c < N; ++c) to_pairs<T>(*reinterpret_cast<Pair(*)[V / 2]>(&v[c * V / 2]), x[k][c]);
+        if (args.threshold != 0) drop_pairs<4>(v, gen, block * 8, args);
 #pragma unroll
-                for (int c = 0; c < N; ++c) unpack_pack(*reinterpret_cast<float(*)[V]>(&v[c * V]), *reinterpret_cast<const Pack<T, V>*>(&x[k][c]));
-                if (args.threshold != 0) apply_block(v, gen.block(static_cast<std::uint32_t>(block)), args.threshold, args.scale);
+        for (int c = 0; c < N; ++c) {
+            Pair(&part)[V / 2] = *reinterpret_cast<Pair(*)[V / 2]>(&v[c * V / 2]);
+            if constexpr (RESIDUAL) {
+                Pair res[V / 2];
+                to_pairs<T>(res, r[k][c]);
 #pragma unroll
-                for (int c = 0; c < N; ++c) {
-                    if constexpr (RESIDUAL) {
-                        float res[V];
-                        unpack_pack(res, *reinterpret_cast<const Pack<T, V>*>(&r[k][c]));
+                for (int i = 0; i < V / 2; ++i) part[i] = add2(part[i], res[i]);
+            }
+            *reinterpret_cast<uint4*>(out + block * 8 + c * V) = to_raw<T>(part);
+        }
+    };
+    for (long long block0 = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; block0 < whole; block0 += stride * BLOCKS) {
+        if (block0 + (BLOCKS - 1) * stride < whole) {
 #pragma unroll
-                        for (int i = 0; i < V; ++i) v[c * V + i] += res[i];
-                    }
-                    store_vec<T, V>(out + block * 8 + c * V, *reinterpret_cast<const float(*)[V]>(&v[c * V]));
-                }
+            for (int k = 0; k < BLOCKS; ++k) load(k, block0 + k * stride);
+#pragma unroll
+            for (int k = 0; k < BLOCKS; ++k) finish(k, block0 + k * stride);
+        } else {
+            for (long long block = block0; block < whole; block += stride) {
+                load(0, block);
+                finish(0, block);
             }
         }
     }
@@ -70,13 +74,17 @@ dropout_kernel(T* out, const T* in, const T* residual, long long count, const Dr
     const Philox gen(args);
     const long long stride = static_cast<long long>(gridDim.x) * kThreads * 8;
     for (long long i = (static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x) * 8; i < count; i += stride) {
-        float v[8];
+        Pair p[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = i + k < count ? to_f32<T>(in[i + k]) : 0.f;
-        if (args.threshold != 0) apply_block(v, gen.block(static_cast<std::uint32_t>(i >> 3)), args.threshold, args.scale);
+        for (int k = 0; k < 4; ++k)
+            p[k] = pair(i + 2 * k < count ? to_f32<T>(in[i + 2 * k]) : 0.f, i + 2 * k + 1 < count ? to_f32<T>(in[i + 2 * k + 1]) : 0.f);
+        if (args.threshold != 0) drop_pairs<4>(p, gen, i, args);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (i + k < count) out[i + k] = from_f32<T>(residual != nullptr ? v[k] + to_f32<T>(residual[i + k]) : v[k]);
+        for (int k = 0; k < 8; ++k) {
+            const float2 f = both(p[k >> 1]);
+            const float v = (k & 1) != 0 ? f.y : f.x;
+            if (i + k < count) out[i + k] = from_f32<T>(residual != nullptr ? v + to_f32<T>(residual[i + k]) : v);
+        }
     }
 }
 

@@ -5,16 +5,21 @@
 //
 // Backward. Token ids follow word frequencies: one id can hold a twentieth of all tokens (or, in a padded batch, most of
 // them), so one owner per table row would leave one CTA adding thousands of rows. Here the tokens are sorted by id (stable
-// radix sort, this file) and the SORTED list is cut into chunks of kChunk tokens, one group of threads each: a group adds its
+// radix sort, this file) and the SORTED list is cut into chunks of as many tokens, one group of threads each: a group adds its
 // tokens' rows run by run, several rows in flight. A run inside a chunk is written to the table at once; runs that cross chunks
 // are joined in shared memory within a CTA, and a run that crosses CTAs leaves fp32 partial rows that a last kernel adds. Every
 // sum is taken in an order that follows from the ids alone, so results repeat bit for bit, and no group has more rows than others.
-// Table rows without a token are zeroed by the same launch (their owners look the row up in the sorted list), so the table
-// is written once.
+// The sort takes one cluster of at most 16 SMs and is all latency; the others clear the table meanwhile (65 MB take 20 us, memory
+// takes 3.5 TB/s of writes alone). Rows with tokens are then written twice. Zeroing only the other rows, from a bitmap that the
+// sort fills, while gradient rows are read, was measured slower (51 against 48 us at 32768 tokens, 32000 x 1024 bf16: the hot
+// words of the bitmap cost the sort more than it saves).
 //
-// Memory-bound: backward reads dout once and writes the table once; the sort moves 16 bytes per token and pass.
+// Memory-bound without dropout: backward reads dout once and writes the table once; the sort moves 16 bytes per token and pass.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
+#include "dependent_launch.cuh"
 #include "philox.cuh"
 #include "launch_counter.h"
 
@@ -23,8 +28,9 @@ namespace {
 
 constexpr int kThreads = 128;        // lookup; threads per row at most
 constexpr int kSumThreads = 512;
-constexpr int kChunk = 16;           // sorted tokens per group of threads
-constexpr int kInFlight = 8;         // rows a group loads before it adds them
+constexpr int kMostChunk = 32;       // sorted tokens per group of threads at most
+constexpr int kMostGroups = 8;       // groups per CTA at most
+constexpr int kInFlight = 4;         // rows a group loads before it adds them
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kKeysPerThread = 8;
@@ -32,42 +38,64 @@ constexpr int kSortTile = kSortThreads * kKeysPerThread;
 constexpr int kMaxDigitBits = 9;
 constexpr int kClusterThreads = 1024;
 constexpr int kMaxCluster = 16;
+constexpr int kMostKeys = 4;         // keys per thread of the cluster sort
 
-// kLookups consecutive tokens per group of threads and trip: their ids, then their rows, are loaded together, and the decisions
-// (about 10 instructions an element, most of the kernel's work) are made while the rows are on their way.
+// kLookups consecutive tokens per group of 2^shift threads and trip: their ids, then their rows, are loaded together. What
+// bounds this kernel is the decisions (about 8 of some 12 instructions an element), which are made while rows are on their way.
 constexpr int kLookups = 4;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
 scaled_embedding_forward_kernel(T* __restrict__ out, const std::uint32_t* __restrict__ ids, const T* __restrict__ weight,
-                                long long tokens, std::uint32_t vocab, int hidden, float scale, int group, const DropoutArgs args) {
+                                long long tokens, std::uint32_t vocab, int hidden, float scale, int shift, const DropoutArgs args) {
     using Raw = typename RawVec<sizeof(T) * VEC>::type;
     const HoistedPhilox gen(args);
-    const int lane = threadIdx.x % group;
-    const long long step = static_cast<long long>(gridDim.x) * (kThreads / group) * kLookups;
-    for (long long t0 = (static_cast<long long>(blockIdx.x) * (kThreads / group) + threadIdx.x / group) * kLookups; t0 < tokens; t0 += step) {
+    const float factor = scale * args.scale;
+    const int group = 1 << shift, lane = threadIdx.x & (group - 1);
+    const long long step = static_cast<long long>(gridDim.x) * (kThreads >> shift) * kLookups;
+    // trips are uniform over a warp: its lanes share their decisions where a vector is one element
+    const long long first = (static_cast<long long>(blockIdx.x) * (kThreads >> shift) + (threadIdx.x >> shift)) * kLookups;
+    const long long warp_first = (static_cast<long long>(blockIdx.x) * (kThreads >> shift) + ((threadIdx.x & ~31u) >> shift)) * kLookups;
+    for (long long w0 = warp_first, t0 = first; w0 < tokens; w0 += step, t0 += step) {
         std::uint32_t id[kLookups];
 #pragma unroll
         for (int k = 0; k < kLookups; ++k) id[k] = t0 + k < tokens ? ids[t0 + k] : 0xffffffffu;
-        for (int c = lane * VEC; c < hidden; c += group * VEC) {
-            Pack<T, VEC> row[kLookups];
-#pragma unroll
-            for (int k = 0; k < kLookups; ++k)
-                if (id[k] < vocab) *reinterpret_cast<Raw*>(&row[k]) = *reinterpret_cast<const Raw*>(weight + static_cast<long long>(id[k]) * hidden + c);
+        for (int c0 = 0; c0 < hidden; c0 += group * VEC) {
+            const int c = c0 + lane * VEC;
+            const bool in = c < hidden;
+            Raw row[kLookups];
 #pragma unroll
             for (int k = 0; k < kLookups; ++k) {
-                if (t0 + k < tokens) {
-                    const long long e = (t0 + k) * hidden + c;
-                    float v[VEC];
-                    if (id[k] < vocab) {
-                        unpack_pack(v, row[k]);
+                row[k] = Raw{};                               // an id outside the table gives zeros
+                if (in && id[k] < vocab) row[k] = *reinterpret_cast<const Raw*>(weight + static_cast<long long>(id[k]) * hidden + c);
+            }
+            T* to = out + t0 * hidden + c;
+            if constexpr (VEC > 1) {
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) v[i] *= scale;
-                        if (args.threshold != 0) drop_vec<VEC>(v, gen, e, args);
-                    } else {
+                for (int k = 0; k < kLookups; ++k) {
+                    if (in && t0 + k < tokens) {
+                        Pair v[VEC / 2];
+                        to_pairs<T>(v, row[k]);
+                        if (args.threshold != 0) drop_pairs<VEC / 2, false>(v, gen, (t0 + k) * hidden + c, args);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+                        for (int i = 0; i < VEC / 2; ++i) v[i] = mul2(v[i], pair(factor));
+                        *reinterpret_cast<uint4*>(to + static_cast<long long>(k) * hidden) = to_raw<T>(v);
                     }
-                    store_vec<T, VEC>(out + e, v);
+                }
+            } else {
+                std::uint32_t kept = 15u;
+                if (args.threshold != 0 && shift >= 5) {
+                    long long start[kLookups];
+#pragma unroll
+                    for (int k = 0; k < kLookups; ++k) start[k] = (t0 + k) * hidden + c - static_cast<int>(threadIdx.x & 31);
+                    kept = keep_four_runs(start, gen, args.threshold);
+                }
+#pragma unroll
+                for (int k = 0; k < kLookups; ++k) {
+                    if (in && t0 + k < tokens) {
+                        float v = to_f32<T>(*reinterpret_cast<const T*>(&row[k])) * factor;
+                        if (args.threshold != 0) v = shift >= 5 ? ((kept >> k) & 1u ? v : 0.f) : apply_one<false>(v, gen, (t0 + k) * hidden + c, args);
+                        to[static_cast<long long>(k) * hidden] = from_f32<T>(v);
+                    }
                 }
             }
         }
@@ -85,7 +113,7 @@ struct SortPass {
     std::uint32_t* vals_out;
     std::uint32_t* counts;           // [1 << bits][tiles]
     std::uint32_t* totals;           // [1 << bits]
-    std::uint32_t* crossing;         // [0]: number of runs that cross a chunk border; cleared by the first pass
+    std::uint32_t* crossing;         // [0]: number of runs that cross a CTA border; cleared by the first pass
     long long n;
     std::uint32_t vocab, skip_id;    // ids >= vocab and skip_id sort behind the table as key `vocab`
     int shift, bits, tiles;
@@ -144,6 +172,18 @@ sort_prefix_kernel(const SortPass p) {
     if (threadIdx.x == 0) p.totals[blockIdx.x] = carry;
 }
 
+// Lanes of the warp that are `in` and have this lane's digit: one vote per bit of the digit, whatever the digits are (a match
+// instruction takes as long as there are different values in the warp, six times as long for the low digit of token ids).
+__device__ __forceinline__ unsigned same_digit(std::uint32_t digit, bool in, int bits) {
+    unsigned peers = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+    for (int b = 0; b < kMaxDigitBits; ++b) {
+        const unsigned set = __ballot_sync(0xffffffffu, (digit >> b) & 1u);
+        if (b < bits) peers &= (digit >> b) & 1u ? set : ~set;
+    }
+    return peers;
+}
+
 __global__ void __launch_bounds__(kSortThreads)
 sort_scatter_kernel(const SortPass p) {
     __shared__ std::uint32_t seen[kSortWarps][1 << kMaxDigitBits];   // keys of a digit met so far by each warp, then its base
@@ -160,9 +200,8 @@ sort_scatter_kernel(const SortPass p) {
         const long long i = base + j * 32;
         const bool in = i < p.n;
         key[j] = in ? sort_key(p, i) : 0u;
-        // keys past the end get a digit of their own, which nobody counts
-        const std::uint32_t digit = in ? (key[j] >> p.shift) & (radix - 1) : 0xffffffffu;
-        const unsigned peers = __match_any_sync(0xffffffffu, digit);
+        const std::uint32_t digit = (key[j] >> p.shift) & (radix - 1);
+        const unsigned peers = same_digit(digit, in, p.bits);
         const unsigned below = __popc(peers & ((1u << lane) - 1u));
         const std::uint32_t so_far = in ? seen[warp][digit] : 0u;
         rank[j] = so_far + below;
@@ -213,31 +252,56 @@ sort_scatter_kernel(const SortPass p) {
     }
 }
 
-// The whole sort in one launch, for up to kMaxCluster * kClusterThreads * KEYS tokens: one cluster holds all keys in registers,
-// digit counts go round in distributed shared memory, keys of a pass through global memory (L2). A pass is then two cluster
-// barriers instead of three launches.
+// The whole sort in one launch, for up to kMaxCluster * kClusterThreads * KEYS tokens: the CTAs of one cluster hold a share of the
+// keys each. Digit counts and, between passes, keys go round in distributed shared memory; only the last pass writes to global
+// memory. A pass is then two cluster barriers instead of three launches. The other clusters of the launch clear memory.
 struct ClusterSort {
+    uint4* clear;                       // memory that the other clusters set to zero
+    long long clear_vectors;            // 16-byte vectors of it; `clear_tail` bytes more behind them
+    int clear_tail;
     const std::uint32_t* ids;
-    std::uint32_t *keys[2], *vals[2];   // pass i writes [i & 1]
-    std::uint32_t* crossing;
+    std::uint32_t *keys, *vals, *crossing;
     int n, bits, passes;
     std::uint32_t vocab, skip_id;
 };
 
 template <int KEYS>
+struct alignas(16) ClusterSmem {
+    static constexpr int kWarps = kClusterThreads / 32, kShare = kClusterThreads * KEYS;   // keys per CTA
+    std::uint32_t key[kShare], val[kShare];                  // the CTA's share in the order of the last pass; written by the whole cluster
+    std::uint32_t mine[1 << kMaxDigitBits];                  // the CTA's keys of each digit; read by the whole cluster
+    std::uint32_t base[1 << kMaxDigitBits];
+    std::uint32_t warp_total[kWarps];
+    alignas(16) unsigned short seen[kWarps][1 << kMaxDigitBits];   // keys of a digit met so far by each warp, then those of earlier warps
+    unsigned short sums[kClusterThreads];                    // [share of the warps][digit]
+};
+
+template <int KEYS>
 __global__ void __launch_bounds__(kClusterThreads)
 sort_cluster_kernel(const ClusterSort p) {
-    constexpr int kWarps = kClusterThreads / 32;
-    __shared__ unsigned short seen[kWarps][1 << kMaxDigitBits];   // keys of a digit met so far by each warp, then those of earlier warps
-    __shared__ std::uint32_t mine[1 << kMaxDigitBits];            // the CTA's keys of each digit; read by the whole cluster
-    __shared__ std::uint32_t base[1 << kMaxDigitBits];
-    __shared__ std::uint32_t warp_total[kWarps];
+    extern __shared__ __align__(16) unsigned char cluster_smem[];
+    using Smem = ClusterSmem<KEYS>;
+    Smem& sm = *reinterpret_cast<Smem*>(cluster_smem);
+    constexpr int kWarps = Smem::kWarps;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
+    launch_dependents();
+    if (blockIdx.x >= cluster.num_blocks()) {
+        const long long workers = static_cast<long long>(gridDim.x - cluster.num_blocks()) * kClusterThreads;
+        long long i = static_cast<long long>(blockIdx.x - cluster.num_blocks()) * kClusterThreads + threadIdx.x;
+        if (i < p.clear_tail) reinterpret_cast<unsigned char*>(p.clear + p.clear_vectors)[i] = 0;
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        for (; i + 7 * workers < p.clear_vectors; i += 8 * workers) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p.clear[i + k * workers] = zero;
+        }
+        for (; i < p.clear_vectors; i += workers) p.clear[i] = zero;
+        return;
+    }
     const int ctas = static_cast<int>(cluster.num_blocks()), cta = static_cast<int>(cluster.block_rank());
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int radix = 1 << p.bits;
-    const int first = (cta * kWarps + warp) * (32 * KEYS) + lane;  // order of the keys: (CTA, warp, j, lane)
+    const int local = warp * (32 * KEYS) + lane, first = cta * Smem::kShare + local;   // order of the keys: (CTA, warp, j, lane)
     if (cta == 0 && threadIdx.x == 0) *p.crossing = 0;
     std::uint32_t key[KEYS], val[KEYS], rank[KEYS];
 #pragma unroll
@@ -249,46 +313,49 @@ sort_cluster_kernel(const ClusterSort p) {
     }
     for (int pass = 0; pass < p.passes; ++pass) {
         const int shift = pass * p.bits;
-        if (pass > 0) {
-#pragma unroll
-            for (int j = 0; j < KEYS; ++j) {
-                const int i = first + j * 32;
-                key[j] = i < p.n ? __ldcg(p.keys[(pass - 1) & 1] + i) : 0u;
-                val[j] = i < p.n ? __ldcg(p.vals[(pass - 1) & 1] + i) : 0u;
-            }
-        }
-        for (int d = lane; d < radix; d += 32) seen[warp][d] = 0;
+        for (int d = lane; d < radix / 8; d += 32) reinterpret_cast<uint4*>(sm.seen[warp])[d] = make_uint4(0u, 0u, 0u, 0u);
+        if (radix < 8 && lane < radix) sm.seen[warp][lane] = 0;
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < KEYS; ++j) {
             const bool in = first + j * 32 < p.n;
-            // keys past the end get a digit of their own, which nobody counts
-            const std::uint32_t digit = in ? (key[j] >> shift) & (radix - 1) : 0xffffffffu;
-            const unsigned peers = __match_any_sync(0xffffffffu, digit);
+            const std::uint32_t digit = (key[j] >> shift) & (radix - 1);
+            const unsigned peers = same_digit(digit, in, p.bits);
             const unsigned below = __popc(peers & ((1u << lane) - 1u));
-            const std::uint32_t so_far = in ? seen[warp][digit] : 0u;
+            const std::uint32_t so_far = in ? sm.seen[warp][digit] : 0u;
             rank[j] = so_far + below;
             __syncwarp();
-            if (in && below == 0) seen[warp][digit] = static_cast<unsigned short>(so_far + __popc(peers));
+            if (in && below == 0) sm.seen[warp][digit] = static_cast<unsigned short>(so_far + __popc(peers));
             __syncwarp();
         }
         __syncthreads();
-        if (threadIdx.x < radix) {
+        // Counts of the warps before each warp: kClusterThreads / radix threads per digit take a share of the warps each.
+        const int digit_of = threadIdx.x & (radix - 1), part = threadIdx.x >> p.bits, parts = kClusterThreads >> p.bits;
+        const int share = parts < kWarps ? kWarps / parts : 1;
+        if (part < kWarps) {
             std::uint32_t before = 0;
-#pragma unroll 8
-            for (int w = 0; w < kWarps; ++w) {
-                const std::uint32_t here = seen[w][threadIdx.x];
-                seen[w][threadIdx.x] = static_cast<unsigned short>(before);
+            for (int w = part * share; w < (part + 1) * share; ++w) {
+                const std::uint32_t here = sm.seen[w][digit_of];
+                sm.seen[w][digit_of] = static_cast<unsigned short>(before);
                 before += here;
             }
-            mine[threadIdx.x] = before;
+            sm.sums[part * radix + digit_of] = static_cast<unsigned short>(before);
+        }
+        __syncthreads();
+        if (part < kWarps) {
+            std::uint32_t before = 0;
+            for (int k = 0; k < part; ++k) before += sm.sums[k * radix + digit_of];
+            if (before != 0)
+                for (int w = part * share; w < (part + 1) * share; ++w) sm.seen[w][digit_of] = static_cast<unsigned short>(sm.seen[w][digit_of] + before);
+            if (part == (parts < kWarps ? parts : kWarps) - 1) sm.mine[digit_of] = before + sm.sums[part * radix + digit_of];
         }
         cluster.sync();
         // Digit d of this CTA starts behind all smaller digits and behind digit d of the CTAs before it.
         std::uint32_t all = 0, earlier = 0;
         if (threadIdx.x < radix) {
-            for (int c = 0; c < ctas; ++c) {
-                const std::uint32_t v = cluster.map_shared_rank(mine, c)[threadIdx.x];
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; ++c) {           // unrolled: the remote reads are on their way together
+                const std::uint32_t v = c < ctas ? cluster.map_shared_rank(sm.mine, c)[threadIdx.x] : 0u;
                 all += v;
                 if (c < cta) earlier += v;
             }
@@ -299,24 +366,38 @@ sort_cluster_kernel(const ClusterSort p) {
             const std::uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += u;
         }
-        if (lane == 31) warp_total[warp] = inc;
+        if (lane == 31) sm.warp_total[warp] = inc;
         __syncthreads();
         if (threadIdx.x < radix) {
             std::uint32_t smaller = 0;
-            for (int w = 0; w < warp; ++w) smaller += warp_total[w];
-            base[threadIdx.x] = smaller + inc - all + earlier;
+            for (int w = 0; w < warp; ++w) smaller += sm.warp_total[w];
+            sm.base[threadIdx.x] = smaller + inc - all + earlier;
         }
         __syncthreads();
-        std::uint32_t *keys_out = p.keys[pass & 1], *vals_out = p.vals[pass & 1];
+        const bool last = pass + 1 == p.passes;
 #pragma unroll
         for (int j = 0; j < KEYS; ++j) {
             if (first + j * 32 < p.n) {
-                const std::uint32_t digit = (key[j] >> shift) & (radix - 1), to = base[digit] + seen[warp][digit] + rank[j];
-                keys_out[to] = key[j];
-                vals_out[to] = val[j];
+                const std::uint32_t digit = (key[j] >> shift) & (radix - 1), to = sm.base[digit] + sm.seen[warp][digit] + rank[j];
+                if (last) {
+                    p.keys[to] = key[j];
+                    p.vals[to] = val[j];
+                } else {
+                    Smem* there = cluster.map_shared_rank(&sm, to / Smem::kShare);
+                    there->key[to % Smem::kShare] = key[j];
+                    there->val[to % Smem::kShare] = val[j];
+                }
             }
         }
-        cluster.sync();   // keys of this pass are written, counts of this pass read
+        // The keys of this pass have arrived, the counts have been read; after the last pass nobody is still being read from.
+        cluster.sync();
+        if (!last) {
+#pragma unroll
+            for (int j = 0; j < KEYS; ++j) {
+                key[j] = sm.key[local + j * 32];
+                val[j] = sm.val[local + j * 32];
+            }
+        }
     }
 }
 
@@ -328,9 +409,9 @@ struct GradArgs {
     std::uint32_t* crossing;         // [0]: count, [1..]: CTAs in which a run starts that goes on in the next CTA
     long long n, hidden;
     std::uint32_t vocab;
-    int ctas, accumulate;            // CTAs of the sum launch that hold tokens
-    int group, groups;               // threads per row, groups per CTA
-    float scale;
+    int ctas, accumulate;
+    int shift, groups, chunk;        // 2^shift threads per row, groups per CTA, tokens per group
+    float scale;                     // of the lookup times that of kept elements
 };
 
 template <typename T, int VEC>
@@ -366,115 +447,107 @@ __device__ __forceinline__ void add_floats(float (&v)[VEC], const float* from) {
     }
 }
 
-// First position of the sorted list whose id is not below `id`.
-__device__ __forceinline__ long long lower_bound(const std::uint32_t* ids, long long n, std::uint32_t id) {
-    long long lo = 0, hi = n;
-    while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if (ids[mid] < id) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
-
-// CTAs [0, g.ctas): g.groups chunks each. The others zero the table rows that no token has, 32 rows per warp.
+// g.groups chunks of g.chunk sorted tokens per CTA.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads, 2)
 scaled_embedding_sum_kernel(T* dw, const T* __restrict__ dout, const GradArgs g, const DropoutArgs args) {
-    extern __shared__ __align__(16) float parts[];           // [groups][2][group * VEC]: what a chunk's first and last run leave
-    __shared__ std::uint32_t ids[kSumThreads * kChunk / 8 + 2], tokens[kSumThreads * kChunk / 8];
-    const int lane = threadIdx.x % g.group, group = threadIdx.x / g.group;
-    if (blockIdx.x >= static_cast<unsigned>(g.ctas)) {
-        const int wl = threadIdx.x & 31;
-        const long long first = (static_cast<long long>(blockIdx.x - g.ctas) * (blockDim.x / 32) + (threadIdx.x >> 5)) * 32;
-        const long long row = first + wl;
-        bool empty = false;
-        if (row < g.vocab) {
-            const long long at = lower_bound(g.ids, g.n, static_cast<std::uint32_t>(row));
-            empty = at == g.n || g.ids[at] != static_cast<std::uint32_t>(row);
-        }
-        unsigned todo = __ballot_sync(0xffffffffu, empty);
-        const float zero[VEC] = {};
-        while (todo != 0) {
-            const int r = __ffs(todo) - 1;
-            todo &= todo - 1;
-            for (long long c = static_cast<long long>(wl) * VEC; c < g.hidden; c += 32 * VEC) store_vec<T, VEC>(dw + (first + r) * g.hidden + c, zero);
-        }
-        return;
-    }
+    extern __shared__ __align__(16) float parts[];           // [threads / per_row][2][per_row * VEC]: what a chunk's first and last run leave
+    const int per_row = 1 << g.shift, lane = threadIdx.x & (per_row - 1), group = threadIdx.x >> g.shift;
+    const int span = g.groups * g.chunk;
+    std::uint32_t* ids = reinterpret_cast<std::uint32_t*>(parts + 2 * VEC * blockDim.x);   // [4 + span + 4]
+    std::uint32_t* tokens = ids + span + 8;                                                 // [span]
     const HoistedPhilox gen(args);
-    // The CTA's tokens, with one id before and one behind them; no neighbour: an id that no token has (vocab marks skipped ones).
-    const int span = g.groups * kChunk;
+    launch_dependents();
+    wait_for_previous();
+    // The CTA's ids and the ones before and behind them; what is not there counts as skipped (id `vocab`, token 0).
     const long long lo = static_cast<long long>(blockIdx.x) * span;
     const int count = g.n - lo < span ? static_cast<int>(g.n - lo) : span;
-    constexpr std::uint32_t kNone = 0xffffffffu;
-    for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
-        const long long at = lo + i - 1;
-        ids[i] = at >= 0 && at < g.n ? g.ids[at] : kNone;
-        if (i < count) tokens[i] = g.tokens[lo + i];
+    for (int i = static_cast<int>(threadIdx.x) - 1; i < span + 1; i += blockDim.x) {
+        const long long at = lo + i;
+        ids[4 + i] = at >= 0 && at < g.n ? g.ids[at] : g.vocab;
+        if (i >= 0 && i < span) tokens[i] = at < g.n ? g.tokens[at] : 0u;
     }
     __syncthreads();
-    const std::uint32_t* id_at = ids + 1;                     // id_at[-1] .. id_at[count]
+    const std::uint32_t* id_at = ids + 4;                     // id_at[-1] .. id_at[span]
     const bool first_from_before = id_at[-1] == id_at[0], last_goes_on = id_at[count] == id_at[count - 1];
     const bool single = id_at[0] == id_at[count - 1];         // all of the CTA's tokens have one id
     if (threadIdx.x == 0 && last_goes_on && id_at[count - 1] < g.vocab && !(single && first_from_before))
         g.crossing[1 + atomicAdd(g.crossing, 1u)] = blockIdx.x;   // their order changes no result
     float* before = g.partial + static_cast<long long>(blockIdx.x) * 2 * g.hidden;
     float* after = before + g.hidden;
-    const int width = g.group * VEC;
+    const int width = per_row * VEC;
     float* head = parts + group * 2 * width + lane * VEC;
     float* tail = head + width;
-    const int begin = group * kChunk, end = begin + kChunk < count ? begin + kChunk : count;
+    const int begin = group * g.chunk, end = begin + g.chunk;
     for (long long c0 = 0; c0 < g.hidden; c0 += width) {
         const long long c = c0 + lane * VEC;
-        if (c < g.hidden && begin < end) {
-            float acc[VEC] = {};
-            std::uint32_t id = id_at[begin];
-            bool open = id_at[begin - 1] == id;               // the run began in an earlier chunk
-            for (int p0 = begin; p0 < end; p0 += kInFlight) {
-                Pack<T, VEC> rows[kInFlight];
-                using Raw = typename RawVec<sizeof(T) * VEC>::type;
+        const bool in = c < g.hidden;
+        float acc[VEC] = {};
+        const bool works = begin < span;                      // threads beyond the groups only join in with the warp
+        std::uint32_t id = works ? id_at[begin] : g.vocab;
+        bool open = works && id_at[begin - 1] == id;          // the run began in an earlier chunk
+        for (int p0 = begin; p0 < begin + g.chunk; p0 += kInFlight) {
+            using Raw = typename RawVec<sizeof(T) * VEC>::type;
+            const uint4 at4 = works ? *reinterpret_cast<const uint4*>(id_at + p0) : make_uint4(g.vocab, g.vocab, g.vocab, g.vocab);
+            const uint4 token4 = works ? *reinterpret_cast<const uint4*>(tokens + p0) : make_uint4(0u, 0u, 0u, 0u);
+            const std::uint32_t at[kInFlight] = {at4.x, at4.y, at4.z, at4.w}, token[kInFlight] = {token4.x, token4.y, token4.z, token4.w};
+            Raw rows[kInFlight];
 #pragma unroll
-                for (int u = 0; u < kInFlight; ++u)
-                    if (p0 + u < end && id_at[p0 + u] < g.vocab)
-                        *reinterpret_cast<Raw*>(&rows[u]) = __ldcs(reinterpret_cast<const Raw*>(dout + static_cast<long long>(tokens[p0 + u]) * g.hidden + c));
+            for (int u = 0; u < kInFlight; ++u)               // without conditions: token 0 stands in past the end
+                rows[u] = __ldcs(reinterpret_cast<const Raw*>(dout + static_cast<long long>(token[u]) * g.hidden + (in ? c : 0)));
+            std::uint32_t kept = 15u;
+            if constexpr (VEC == 1) {
+                if (args.threshold != 0 && g.shift >= 5) {
+                    long long start[kInFlight];
 #pragma unroll
-                for (int u = 0; u < kInFlight; ++u) {
-                    if (p0 + u < end) {
-                        const std::uint32_t next = id_at[p0 + u];
-                        if (next != id) {
-                            if (open) put_floats<VEC>(head, acc);
-                            else write_row<T, VEC>(dw + static_cast<long long>(id) * g.hidden + c, acc, g.scale, g.accumulate);
+                    for (int u = 0; u < kInFlight; ++u) start[u] = static_cast<long long>(token[u]) * g.hidden + c - static_cast<int>(threadIdx.x & 31);
+                    kept = keep_four_runs(start, gen, args.threshold);
+                }
+            }
 #pragma unroll
-                            for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-                            id = next;
-                            open = false;
+            for (int u = 0; u < kInFlight; ++u) {
+                if (at[u] != id) {                            // never from a skipped token: they are last
+                    if (in && open) put_floats<VEC>(head, acc);
+                    else if (in) write_row<T, VEC>(dw + static_cast<long long>(id) * g.hidden + c, acc, g.scale, g.accumulate);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+                    id = at[u];
+                    open = false;
+                }
+                {                                             // skipped tokens are added to a sum that nobody writes
+                    const long long e = static_cast<long long>(token[u]) * g.hidden + c;
+                    if constexpr (VEC > 1) {
+                        Pair v[VEC / 2];
+                        to_pairs<T>(v, rows[u]);
+                        if (args.threshold != 0) drop_pairs<VEC / 2, false>(v, gen, e, args);
+#pragma unroll
+                        for (int i = 0; i < VEC / 2; ++i) {
+                            const float2 s = both(add2(pair(acc[2 * i], acc[2 * i + 1]), v[i]));
+                            acc[2 * i] = s.x;
+                            acc[2 * i + 1] = s.y;
                         }
-                        if (next < g.vocab) {
-                            float v[VEC];
-                            unpack_pack(v, rows[u]);
-                            if (args.threshold != 0) drop_vec<VEC>(v, gen, static_cast<long long>(tokens[p0 + u]) * g.hidden + c, args);
-#pragma unroll
-                            for (int i = 0; i < VEC; ++i) acc[i] += v[i];
-                        }
+                    } else {
+                        float v = to_f32<T>(*reinterpret_cast<const T*>(&rows[u]));
+                        if (args.threshold != 0) v = g.shift >= 5 ? ((kept >> u) & 1u ? v : 0.f) : apply_one<false>(v, gen, e, args);
+                        acc[0] += v;
                     }
                 }
             }
-            if (id < g.vocab) {
-                if (open) put_floats<VEC>(head, acc);         // also where the whole chunk is one run that goes on
-                else if (id_at[end] == id) put_floats<VEC>(tail, acc);
-                else write_row<T, VEC>(dw + static_cast<long long>(id) * g.hidden + c, acc, g.scale, g.accumulate);
-            }
+        }
+        if (in && id < g.vocab) {
+            if (open) put_floats<VEC>(head, acc);             // also where the whole chunk is one run that goes on
+            else if (id_at[end] == id) put_floats<VEC>(tail, acc);
+            else write_row<T, VEC>(dw + static_cast<long long>(id) * g.hidden + c, acc, g.scale, g.accumulate);
         }
         __syncthreads();
         // Runs that cross chunks: the threads of group 0 (more, where a group has few) walk over the CTA's chunks in order.
-        for (int k = threadIdx.x; k < g.group; k += blockDim.x) {
+        for (int k = threadIdx.x; k < per_row; k += blockDim.x) {
             const long long col = c0 + k * VEC;
             if (col >= g.hidden) continue;
             float acc[VEC] = {};
             bool carried = false, from_before = false;
-            for (int q = 0; q * kChunk < count; ++q) {
-                const int b = q * kChunk, e = b + kChunk < count ? b + kChunk : count;
+            for (int q = 0; q < g.groups; ++q) {
+                const int b = q * g.chunk, e = b + g.chunk;
                 const std::uint32_t id0 = id_at[b], id1 = id_at[e - 1];
                 if (id0 >= g.vocab) break;
                 const float* part = parts + q * 2 * width + k * VEC;
@@ -508,22 +581,19 @@ __global__ void __launch_bounds__(kJoinThreads)
 scaled_embedding_join_kernel(T* dw, const GradArgs g) {
     __shared__ float tile[kJoinThreads / 32][32 * VEC];
     const int lane = threadIdx.x & 31, pl = threadIdx.x >> 5;
+    wait_for_previous();
     const unsigned column_tiles = static_cast<unsigned>((g.hidden + 32 * VEC - 1) / (32 * VEC)), runs = *g.crossing;
-    const int span = g.groups * kChunk;
+    const long long span = static_cast<long long>(g.groups) * g.chunk;
     for (unsigned run = blockIdx.x / column_tiles; run < runs; run += gridDim.x / column_tiles) {
         const long long cta = g.crossing[1 + run];
         const long long col = (static_cast<long long>(blockIdx.x % column_tiles) * 32 + lane) * VEC;
         const std::uint32_t id = g.ids[cta * span + span - 1];
-        // last CTA whose first token belongs to the run
-        long long lo = cta + 1, hi = g.ctas - 1;
-        for (long long reach = 1; lo + reach <= hi && g.ids[(lo + reach) * span] == id; reach *= 2) lo += reach;   // most runs are short
-        if (lo + 1 < hi + 1) {
-            long long top = hi;
-            while (lo < top) {
-                const long long mid = (lo + top + 1) >> 1;
-                if (g.ids[mid * span] == id) lo = mid;
-                else top = mid - 1;
-            }
+        // last CTA whose first token belongs to the run, looked for 32 CTAs at a time
+        long long lo = cta;
+        unsigned alike = 0xffffffffu;
+        while (alike == 0xffffffffu) {
+            alike = __ballot_sync(0xffffffffu, lo + 1 + lane < g.ctas && g.ids[(lo + 1 + lane) * span] == id);
+            lo += alike == 0xffffffffu ? 32 : __ffs(~alike) - 1;
         }
         float acc[VEC] = {};
         if (col < g.hidden)
@@ -546,26 +616,31 @@ int bit_length(std::uint64_t v) {
     return b;
 }
 
-// Threads per row: enough for the row's vectors, at most kThreads.
-int group_for(std::size_t hidden, int vec) {
-    int g = 1;
-    while (g < kThreads && static_cast<std::size_t>(g) * vec < hidden) g *= 2;
-    return g;
+// Threads per row, as a power of two: enough for the row's vectors, at most kThreads.
+int group_shift(std::size_t hidden, int vec) {
+    int s = 0;
+    while ((1 << s) < kThreads && (std::size_t{1} << s) * vec < hidden) ++s;
+    return s;
 }
 
-// Layout of the run sums: threads per row, groups per CTA, CTAs.
+std::size_t at_most(std::size_t n, std::size_t limit) { return n < limit ? n : limit; }
+
+// Layout of the run sums: threads per row (2^shift), groups per CTA, CTAs.
 struct SumPlan {
-    int group, groups, ctas;
+    int shift, groups, chunk, ctas;
     SumPlan(std::size_t tokens, std::size_t hidden, int vec) {
-        group = group_for(hidden, vec);
-        // As many groups as threads (and the staged ids) allow, fewer when there are few tokens: then every SM gets some.
-        const std::size_t chunks = (tokens + kChunk - 1) / kChunk, share = (chunks + 2 * kNumSMs - 1) / (2 * kNumSMs);
-        std::size_t n = kSumThreads / (group < 8 ? 8 : group);
-        const std::size_t whole_warps = group < 32 ? 32 / group : 1;
-        if (n > share) n = share;
-        n = n < whole_warps ? whole_warps : n / whole_warps * whole_warps;
+        shift = group_shift(hidden, vec);
+        const std::size_t group = std::size_t{1} << shift;
+        // As many groups as threads allow (and kMostGroups, whose runs are joined one after the other), fewer when there are few
+        // tokens: then every SM gets some. Chunks
+        // as long as lets all CTAs run at once (two per SM), up to kMostChunk.
+        const std::size_t slots = 2 * kNumSMs;
+        std::size_t n = at_most(kSumThreads / group, kMostGroups);
+        n = at_most(n, (tokens + slots * kInFlight - 1) / (slots * kInFlight));
         groups = static_cast<int>(n);
-        ctas = static_cast<int>((chunks + n - 1) / n);
+        const std::size_t even = (tokens + slots * n - 1) / (slots * n);
+        chunk = static_cast<int>(even < kMostChunk ? (even + kInFlight - 1) / kInFlight * kInFlight : kMostChunk);
+        ctas = static_cast<int>((tokens + n * chunk - 1) / (n * chunk));
     }
 };
 
@@ -602,42 +677,50 @@ bool valid_sizes(std::size_t tokens, std::size_t vocab, std::size_t hidden) {
 template <typename T, int VEC>
 int launch_sum(void* dw, const void* dout, GradArgs g, const DropoutArgs& args, cudaStream_t s) {
     const SumPlan p(static_cast<std::size_t>(g.n), static_cast<std::size_t>(g.hidden), VEC);
-    g.group = p.group;
+    g.shift = p.shift;
     g.groups = p.groups;
+    g.chunk = p.chunk;
     g.ctas = p.ctas;
-    const int threads = g.groups * g.group;
-    const unsigned zero_ctas = g.accumulate ? 0 : static_cast<unsigned>((g.vocab + threads - 1ull) / threads);
-    const std::size_t smem = static_cast<std::size_t>(g.groups) * 2 * g.group * VEC * sizeof(float);
-    scaled_embedding_sum_kernel<T, VEC><<<g.ctas + zero_ctas, threads, smem, s>>>(static_cast<T*>(dw), static_cast<const T*>(dout), g, args);
+    const int threads = g.groups << g.shift < 32 ? 32 : g.groups << g.shift;
+    const std::size_t smem = static_cast<std::size_t>(threads) * 2 * VEC * sizeof(float) + (2 * static_cast<std::size_t>(g.groups) * g.chunk + 8) * 4;
+    static PerDeviceOnce once;
+    if (once.needed()) {
+        CGPT_CUDA_TRY(cudaFuncSetAttribute(scaled_embedding_sum_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+        once.done();
+    }
+    CGPT_CUDA_TRY(launch_after_previous(scaled_embedding_sum_kernel<T, VEC>, dim3(g.ctas), threads, smem, s, static_cast<T*>(dw), static_cast<const T*>(dout), g, args));
     count_launch();
-    CGPT_LAUNCH_CHECK();
     if (g.ctas == 1) return CGPT_OK;
     constexpr int JV = VEC < 4 ? 1 : 4;
     const unsigned column_tiles = static_cast<unsigned>((g.hidden + 32 * JV - 1) / (32 * JV));
-    const unsigned runs = g.ctas - 1, lanes = column_tiles < kNumSMs * 8u ? kNumSMs * 8u / column_tiles : 1;   // runs at a time
-    scaled_embedding_join_kernel<T, JV><<<column_tiles * (runs < lanes ? runs : lanes), kJoinThreads, 0, s>>>(static_cast<T*>(dw), g);
+    const unsigned runs = g.ctas - 1, lanes = column_tiles < kNumSMs * 32u ? kNumSMs * 32u / column_tiles : 1;   // runs at a time
+    CGPT_CUDA_TRY(launch_after_previous(scaled_embedding_join_kernel<T, JV>, dim3(column_tiles * (runs < lanes ? runs : lanes)), kJoinThreads, 0, s,
+                                        static_cast<T*>(dw), g));
     count_launch();
-    CGPT_LAUNCH_CHECK();
     return CGPT_OK;
 }
 
-constexpr std::size_t kClusterTokens = std::size_t{8} * kMaxCluster * kClusterThreads;
+constexpr std::size_t kClusterTokens = std::size_t{kMostKeys} * kMaxCluster * kClusterThreads;
 
 // One launch of one cluster, up to kClusterTokens tokens.
 int launch_cluster_sort(const ClusterSort& p, cudaStream_t s) {
     int ctas = 1;
     while (ctas < kMaxCluster && ctas * kClusterThreads < p.n) ctas *= 2;
     const int keys = (p.n + ctas * kClusterThreads - 1) / (ctas * kClusterThreads);
-    auto kernel = keys == 1 ? sort_cluster_kernel<1> : keys == 2 ? sort_cluster_kernel<2> : keys <= 4 ? sort_cluster_kernel<4> : sort_cluster_kernel<8>;
-    static PerDeviceOnce once[4];
-    PerDeviceOnce& o = once[keys == 1 ? 0 : keys == 2 ? 1 : keys <= 4 ? 2 : 3];
-    if (o.needed()) {
+    const int size = keys == 1 ? 0 : keys == 2 ? 1 : 2;
+    void (*const kernels[3])(ClusterSort) = {sort_cluster_kernel<1>, sort_cluster_kernel<2>, sort_cluster_kernel<kMostKeys>};
+    constexpr std::size_t smem[3] = {sizeof(ClusterSmem<1>), sizeof(ClusterSmem<2>), sizeof(ClusterSmem<kMostKeys>)};
+    auto kernel = kernels[size];
+    static PerDeviceOnce once[3];
+    if (once[size].needed()) {
         CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        o.done();
+        CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem[size])));
+        once[size].done();
     }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(ctas);
+    config.gridDim = dim3(p.clear != nullptr ? 128 / ctas * ctas : ctas);   // clusters of 16 that fit on the SMs at a time: 8
     config.blockDim = dim3(kClusterThreads);
+    config.dynamicSmemBytes = smem[size];
     config.stream = s;
     cudaLaunchAttribute attribute;
     attribute.id = cudaLaunchAttributeClusterDimension;
@@ -670,11 +753,12 @@ extern "C" int cgpt_scaled_embedding_forward(void* out, const uint32_t* ids, con
         constexpr int V = 16 / sizeof(T);
         const bool vector = hidden % V == 0 && aligned16(out) && aligned16(weight);
         auto kernel = vector ? scaled_embedding_forward_kernel<T, V> : scaled_embedding_forward_kernel<T, 1>;
-        const int group = group_for(hidden, vector ? V : 1);
-        const std::size_t per_cta = static_cast<std::size_t>(kThreads / group) * kLookups, need = (tokens + per_cta - 1) / per_cta;
-        kernel<<<static_cast<unsigned>(need), kThreads, 0, s>>>(
+        const int shift = group_shift(hidden, vector ? V : 1);
+        const std::size_t per_cta = static_cast<std::size_t>(kThreads >> shift) * kLookups, need = (tokens + per_cta - 1) / per_cta;
+        const std::size_t cap = static_cast<std::size_t>(kNumSMs) * resident_ctas_per_sm(reinterpret_cast<const void*>(kernel), kThreads, 0);
+        kernel<<<static_cast<unsigned>(need < cap ? need : cap), kThreads, 0, s>>>(
             static_cast<T*>(out), ids, static_cast<const T*>(weight), static_cast<long long>(tokens), static_cast<std::uint32_t>(vocab),
-            static_cast<int>(hidden), scale, group, args);
+            static_cast<int>(hidden), scale, shift, args);
         count_launch();
         CGPT_LAUNCH_CHECK();
     });
@@ -705,8 +789,26 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
     const int bits = bit_length(vocab);   // keys are in [0, vocab]
     const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     const int digit_bits = (bits + passes - 1) / passes;
-    ClusterSort c{ids, {words(at.keys[0]), words(at.keys[1])}, {words(at.vals[0]), words(at.vals[1])}, words(at.crossing),
-                  static_cast<int>(tokens), digit_bits, passes, static_cast<std::uint32_t>(vocab), padding_id};
+    const std::size_t table_bytes = vocab * hidden * dtype_size(dtype);
+    ClusterSort c{};
+    // The table starts on an element, the vectors that clear it on 16 bytes: the few bytes before go with a small memset.
+    const std::size_t lead = std::min<std::size_t>((16 - (reinterpret_cast<std::uintptr_t>(grad_weight) & 15)) & 15, table_bytes);
+    if (!accumulate) {
+        if (lead != 0 || tokens > kClusterTokens) CGPT_CUDA_TRY(cudaMemsetAsync(grad_weight, 0, tokens > kClusterTokens ? table_bytes : lead, s));
+        c.clear = reinterpret_cast<uint4*>(static_cast<unsigned char*>(grad_weight) + lead);
+        c.clear_vectors = static_cast<long long>((table_bytes - lead) / 16);
+        c.clear_tail = static_cast<int>((table_bytes - lead) % 16);
+    }
+    c.ids = ids;
+    const int last = tokens <= kClusterTokens ? 0 : (passes - 1) & 1;   // which buffers the sorted tokens end up in
+    c.keys = words(at.keys[last]);
+    c.vals = words(at.vals[last]);
+    c.crossing = words(at.crossing);
+    c.n = static_cast<int>(tokens);
+    c.bits = digit_bits;
+    c.passes = passes;
+    c.vocab = static_cast<std::uint32_t>(vocab);
+    c.skip_id = padding_id;
     if (tokens <= kClusterTokens) {
         CGPT_TRY(launch_cluster_sort(c, s));
     } else {
@@ -722,8 +824,8 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
         p.keys_in = ids;
         for (int i = 0; i < passes; ++i) {
             p.shift = i * p.bits;
-            p.keys_out = c.keys[i & 1];
-            p.vals_out = c.vals[i & 1];
+            p.keys_out = words(at.keys[i & 1]);
+            p.vals_out = words(at.vals[i & 1]);
             sort_count_kernel<<<at.tiles, kSortThreads, 0, s>>>(p);
             CGPT_LAUNCH_CHECK();
             sort_prefix_kernel<<<1 << p.bits, kSortThreads, 0, s>>>(p);
@@ -735,9 +837,8 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
             p.vals_in = p.vals_out;
         }
     }
-    const int last = (passes - 1) & 1;
-    const GradArgs g{c.keys[last], c.vals[last], reinterpret_cast<float*>(base + at.partial), c.crossing, static_cast<long long>(tokens),
-                     static_cast<long long>(hidden), c.vocab, 0, accumulate, 0, 0, scale};
+    const GradArgs g{c.keys, c.vals, reinterpret_cast<float*>(base + at.partial), c.crossing, static_cast<long long>(tokens),
+                     static_cast<long long>(hidden), c.vocab, 0, accumulate, 0, 0, 0, scale * args.scale};
     CGPT_DISPATCH_DTYPE(dtype, T, {
         constexpr int V = 16 / sizeof(T);
         if (hidden % V == 0 && aligned16(grad_weight) && aligned16(grad_output)) return (launch_sum<T, V>(grad_weight, grad_output, g, args, s));

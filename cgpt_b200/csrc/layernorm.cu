@@ -14,6 +14,7 @@
 // Memory-bound: 2 * H * sizeof(T) bytes per row forward, 3 backward (+1 with a residual), 4 and 5 for the fused pair.
 #include <type_traits>
 
+#include "dependent_launch.cuh"
 #include "philox.cuh"
 #include "launch_counter.h"
 #include "sm100.cuh"
@@ -196,6 +197,7 @@ __global__ void __launch_bounds__(kThreads)
 layernorm_columns_any_kernel(float* __restrict__ partial, const T* __restrict__ dy, const T* __restrict__ x,
                              const float2* __restrict__ stats, long long rows, long long hidden) {
     __shared__ float tile[2][kWarps][33];
+    launch_dependents();
     const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = static_cast<long long>(blockIdx.x) * 32 + lane;
     const long long share = (rows + gridDim.y - 1) / gridDim.y;
@@ -229,6 +231,7 @@ layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __r
     const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = static_cast<long long>(blockIdx.x) * 32 + lane;
     float acc = 0.f;
+    wait_for_previous();
     if (col < hidden)
         for (int p = rl; p < parts; p += 32) acc += partial[(static_cast<long long>(p) * 2 + blockIdx.y) * hidden + col];
     tile[rl][lane] = acc;
@@ -433,10 +436,9 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
     float* partial = static_cast<float*>(workspace);
     const unsigned columns = static_cast<unsigned>((hidden + 31) / 32);
     auto reduce = [&](std::size_t parts) {
-        layernorm_reduce_kernel<T><<<dim3(columns, db != nullptr ? 2 : 1), 1024, 0, s>>>(
-            static_cast<T*>(dw), static_cast<T*>(db), partial, static_cast<int>(parts), static_cast<long long>(hidden));
+        CGPT_CUDA_TRY(launch_after_previous(layernorm_reduce_kernel<T>, dim3(columns, db != nullptr ? 2 : 1), 1024, 0, s, static_cast<T*>(dw),
+                                            static_cast<T*>(db), partial, static_cast<int>(parts), static_cast<long long>(hidden)));
         count_launch();
-        CGPT_LAUNCH_CHECK();
         return CGPT_OK;
     };
     const bool al = aligned16(dx) && aligned16(din) && aligned16(dy) && aligned16(x) && aligned16(w) && aligned16(residual);

@@ -27,96 +27,6 @@ constexpr std::size_t kStatsBytes = 2 * kMaxTileRows * 32;   // static shared me
 // Rows a warp group takes at a time: a lane with few vectors per row holds several rows.
 __host__ __device__ constexpr int rows_at_once(int cpt) { return cpt >= 4 ? 1 : 4 / cpt; }
 
-using Pair = unsigned long long;         // two fp32 values in a 64-bit register
-
-__device__ __forceinline__ Pair pair(float a, float b) {
-    Pair p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
-    return p;
-}
-__device__ __forceinline__ Pair pair(float a) { return pair(a, a); }
-__device__ __forceinline__ float2 both(Pair p) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-    return f;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float halves_sum(Pair p) {
-    const float2 f = both(p);
-    return f.x + f.y;
-}
-
-template <typename T> __device__ __forceinline__ Pair pair_of(std::uint32_t two);
-template <> __device__ __forceinline__ Pair pair_of<__half>(std::uint32_t two) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
-    return pair(f.x, f.y);
-}
-template <> __device__ __forceinline__ Pair pair_of<__nv_bfloat16>(std::uint32_t two) {
-    return pair(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
-}
-template <typename T> __device__ __forceinline__ std::uint32_t two_of(Pair p);
-template <> __device__ __forceinline__ std::uint32_t two_of<__half>(Pair p) {
-    const float2 f = both(p);
-    const __half2 h = __floats2half2_rn(f.x, f.y);
-    return *reinterpret_cast<const std::uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ std::uint32_t two_of<__nv_bfloat16>(Pair p) {
-    const float2 f = both(p);
-    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
-    return *reinterpret_cast<const std::uint32_t*>(&h);
-}
-
-// A 16-byte vector as pairs, and back (one rounding to T).
-template <typename T>
-__device__ __forceinline__ void to_pairs(Pair (&p)[8 / sizeof(T)], const uint4& raw) {
-    if constexpr (sizeof(T) == 4) {
-        p[0] = pair(__uint_as_float(raw.x), __uint_as_float(raw.y));
-        p[1] = pair(__uint_as_float(raw.z), __uint_as_float(raw.w));
-    } else {
-        p[0] = pair_of<T>(raw.x);
-        p[1] = pair_of<T>(raw.y);
-        p[2] = pair_of<T>(raw.z);
-        p[3] = pair_of<T>(raw.w);
-    }
-}
-template <typename T>
-__device__ __forceinline__ uint4 to_raw(const Pair (&p)[8 / sizeof(T)]) {
-    if constexpr (sizeof(T) == 4) {
-        const float2 a = both(p[0]), b = both(p[1]);
-        return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
-    } else {
-        return make_uint4(two_of<T>(p[0]), two_of<T>(p[1]), two_of<T>(p[2]), two_of<T>(p[3]));
-    }
-}
-template <typename T, typename Generator>
-__device__ __forceinline__ void drop_pairs(Pair (&p)[8 / sizeof(T)], const Generator& gen, long long e, const DropoutArgs& args) {
-    constexpr int VEC = 16 / sizeof(T);
-    float v[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-        const float2 f = both(p[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
-    drop_vec<VEC>(v, gen, e, args);
-#pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
-}
-
 // A ring of stages. A wait that runs out sets the library's status word; the CTA then goes on with what is there (every barrier
 // is still met, nothing is written out of bounds) and waits no more.
 struct Ring {
@@ -278,7 +188,7 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
                     to_pairs<T>(v[r][c], *reinterpret_cast<const uint4*>(at + r * next_row + c * 512));
                     if constexpr (FUSED) {
                         const long long e = e0 + r * per_warp * hidden + c * (32 * VEC);
-                        if (args.threshold != 0) drop_pairs<T>(v[r][c], gen, e, args);
+                        if (args.threshold != 0) drop_pairs<NP>(v[r][c], gen, e, args);
                         Pair res[NP];
                         to_pairs<T>(res, *reinterpret_cast<const uint4*>(at + ring.tensor_bytes + r * next_row + c * 512));
 #pragma unroll
@@ -361,6 +271,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     const int per_warp = 32 / ra.lanes;
     const int lane_row = lane / ra.lanes, vec0 = warp_in_row * (32 * CPT) + (lane & (ra.lanes - 1));
     float* red = reinterpret_cast<float*>(shared + kSumsOffset) + unit * 64;
+    launch_dependents();
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
     const long long step = static_cast<long long>(gridDim.x) * ra.step_rows;
     const long long first = static_cast<long long>(blockIdx.x) * ra.step_rows;
@@ -518,7 +429,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
                             }
                             *reinterpret_cast<uint4*>(dx + e) = to_raw<T>(out);
                             if constexpr (FUSED) {
-                                if (args.threshold != 0) drop_pairs<T>(out, gen, e, args);
+                                if (args.threshold != 0) drop_pairs<NP>(out, gen, e, args);
                                 *reinterpret_cast<uint4*>(din + e) = to_raw<T>(out);
                             }
                         }

@@ -38,28 +38,6 @@ __device__ __forceinline__ void group_sum(float (&v)[NV], const Group& g, float*
     W::broadcast(v);
 }
 
-// Decisions for four runs of 32 consecutive elements, one element of each run per lane: bit j of the result belongs to run j,
-// whose lane 0 has element start[j]. A run touches at most 5 generator blocks, so 8 lanes work out the blocks of one run and
-// hand the decisions round: one block per lane and 4 elements, not one per element.
-__device__ __forceinline__ std::uint32_t keep_four_runs(const long long (&start)[4], const Philox& gen, std::uint32_t threshold) {
-    const int lane = threadIdx.x & 31;
-    long long mine = start[0];
-#pragma unroll
-    for (int j = 1; j < 4; ++j)
-        if ((lane >> 3) == j) mine = start[j];
-    const uint4 c = gen.block(static_cast<std::uint32_t>(mine >> 3) + (lane & 7));
-    const std::uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    std::uint32_t kept = 0, out = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) kept |= (((i & 1) != 0 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu) >= threshold ? 1u : 0u) << i;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int at = static_cast<int>(start[j] & 7) + lane;      // element of lane `lane`, counted from the run's first block
-        out |= ((__shfl_sync(0xffffffffu, kept, j * 8 + (at >> 3)) >> (at & 7)) & 1u) << j;
-    }
-    return out;
-}
-
 // R rows of a tensor; zeros past the rows and columns.
 template <typename T, int CPT, int R>
 __device__ __forceinline__ void load_rows(float (&v)[R][CPT], const T* from, long long row0, long long rows, int hidden, int tpr, int tid) {
@@ -164,6 +142,7 @@ layernorm_backward_rows_kernel(T* dx, T* din, float* __restrict__ partial, const
     const Group g{index, tpr >> 5, tid >> 5, static_cast<int>(threadIdx.x & 31)};
     float* red = shared + index * (4 * R * 16);
     const Philox gen(args);
+    launch_dependents();
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
     const int groups = blockDim.x / tpr;
     float aw[CPT] = {}, ab[CPT] = {};

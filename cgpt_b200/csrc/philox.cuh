@@ -16,6 +16,7 @@
 #include <initializer_list>
 
 #include "common.cuh"
+#include "pairs.cuh"
 
 namespace cgpt {
 
@@ -72,45 +73,55 @@ struct PhiloxOf {
 using Philox = PhiloxOf<false>;
 using HoistedPhilox = PhiloxOf<true>;
 
-// One element's decision on the high half of `u` (its low half may hold anything: u >= t * 2^16 exactly if its high half >= t).
-// The product is rounded by itself (no contraction with a residual added to it), so that every kernel gives the same bits.
-__device__ __forceinline__ float decide(float v, std::uint32_t u, std::uint32_t threshold, float scale) {
-    return u >= threshold << 16 ? __fmul_rn(v, scale) : 0.f;
-}
+// Decisions are made on the high half of a word (its low half may hold anything: u >= t * 2^16 exactly if its high half >= t).
+// Products by the scale are rounded by themselves (no contraction with a residual added to them), so that every kernel gives the
+// same bits.
 
-// Applies a block's eight decisions to eight consecutive elements. Dropped elements become +0 whatever they held.
-__device__ __forceinline__ void apply_block(float (&v)[8], const uint4& bits, std::uint32_t threshold, float scale) {
-    const std::uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+// The dropout map of NP pairs that start at element e of the tensor (e % (2 NP) == 0, NP 2 or 4). Dropped elements become +0
+// whatever they held. SCALED: kept elements are multiplied by the scale (else the caller does that later).
+template <int NP, bool SCALED = true, typename Generator>
+__device__ __forceinline__ void drop_pairs(Pair (&p)[NP], const Generator& gen, long long e, const DropoutArgs& args) {
+    const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
+    const bool upper = NP == 2 && (e & 4) != 0;
+    const std::uint32_t w[4] = {upper ? c.z : c.x, upper ? c.w : c.y, c.z, c.w};
+    const Pair scale = pair(args.scale);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = decide(v[i], (i & 1) != 0 ? w[i >> 1] : w[i >> 1] << 16, threshold, scale);
+    for (int i = 0; i < NP; ++i) {
+        const float2 f = both(SCALED ? mul2(p[i], scale) : p[i]);
+        p[i] = pair(w[i] << 16 >= args.threshold << 16 ? f.x : 0.f, w[i] >= args.threshold << 16 ? f.y : 0.f);
+    }
 }
 
 // The decision of one element, for places that cannot share a block (its other seven decisions are thrown away).
-template <typename Generator>
+template <bool SCALED = true, typename Generator>
 __device__ __forceinline__ float apply_one(float v, const Generator& gen, long long e, const DropoutArgs& a) {
     const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
     const int i = static_cast<int>(e & 7);
     const std::uint32_t w = i < 4 ? (i < 2 ? c.x : c.y) : (i < 6 ? c.z : c.w);
-    return decide(v, (i & 1) != 0 ? w : w << 16, a.threshold, a.scale);
+    return ((i & 1) != 0 ? w : w << 16) >= a.threshold << 16 ? (SCALED ? __fmul_rn(v, a.scale) : v) : 0.f;
 }
 
-// The dropout map of VEC elements that start at element e of the tensor (e % VEC == 0 for VEC > 1).
-template <int VEC, typename Generator>
-__device__ __forceinline__ void drop_vec(float (&v)[VEC], const Generator& gen, long long e, const DropoutArgs& args) {
-    if constexpr (VEC == 8) {
-        apply_block(v, gen.block(static_cast<std::uint32_t>(e >> 3)), args.threshold, args.scale);
-    } else if constexpr (VEC == 4) {
-        const uint4 c = gen.block(static_cast<std::uint32_t>(e >> 3));
-        const bool high = (e & 4) != 0;
-        const std::uint32_t w0 = high ? c.z : c.x, w1 = high ? c.w : c.y;
-        v[0] = decide(v[0], w0 << 16, args.threshold, args.scale);
-        v[1] = decide(v[1], w0, args.threshold, args.scale);
-        v[2] = decide(v[2], w1 << 16, args.threshold, args.scale);
-        v[3] = decide(v[3], w1, args.threshold, args.scale);
-    } else {
+// Decisions for four runs of 32 consecutive elements, one element of each run per lane: bit j of the result belongs to run j,
+// whose lane 0 has element start[j]. A run touches at most 5 generator blocks, so 8 lanes work out the blocks of one run and
+// hand the decisions round: one block per lane and 4 elements, not one per element.
+template <typename Generator>
+__device__ __forceinline__ std::uint32_t keep_four_runs(const long long (&start)[4], const Generator& gen, std::uint32_t threshold) {
+    const int lane = threadIdx.x & 31;
+    long long mine = start[0];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = apply_one(v[i], gen, e + i, args);
+    for (int j = 1; j < 4; ++j)
+        if ((lane >> 3) == j) mine = start[j];
+    const uint4 c = gen.block(static_cast<std::uint32_t>(mine >> 3) + (lane & 7));
+    const std::uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    std::uint32_t kept = 0, out = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kept |= (((i & 1) != 0 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu) >= threshold ? 1u : 0u) << i;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int at = static_cast<int>(start[j] & 7) + lane;      // element of lane `lane`, counted from the run's first block
+        out |= ((__shfl_sync(0xffffffffu, kept, j * 8 + (at >> 3)) >> (at & 7)) & 1u) << j;
     }
+    return out;
 }
 
 // Whether every pointer given (NULL ones aside) is aligned to an element of `dtype`.
