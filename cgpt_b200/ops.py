@@ -440,6 +440,7 @@ class ScaledEmbeddingOptions:
 
 
 _NO_DROPOUT = DropoutOptions()
+_STATE_DTYPES = (torch.int64, torch.uint64)
 
 
 def make_dropout_state(seed: int, step: int = 0, device=None) -> torch.Tensor:
@@ -457,35 +458,42 @@ def dropout_advance(state, steps: int = 1, stream=None):
 
 
 def _state_check(name, state, device=None):
-    _require(state is not None and state.is_cuda and state.dtype in (torch.int64, torch.uint64) and state.numel() == 2 and state.is_contiguous()
-             and (device is None or state.get_device() == device), f"{name}: state must be two 64-bit words on the tensors' device")
+    if (state is None or state.dtype not in _STATE_DTYPES or state.numel() != 2 or not state.is_contiguous()
+            or (not state.is_cuda if device is None else state.get_device() != device)):
+        _require(False, f"{name}: state must be two 64-bit words on the tensors' device")
     return state.get_device()
 
 
 def _dropout_options(name, options, state, device):
     """(probability, state pointer, site) of a call."""
     o = options or _NO_DROPOUT
-    _require(0.0 <= o.probability < 1.0, f"{name}: probability must be in [0, 1)")
-    _require(0 <= o.site <= 0xffffffff, f"{name}: site must fit 32 bits")
+    if not (0.0 <= o.probability < 1.0 and 0 <= o.site <= 0xffffffff):
+        _require(False, f"{name}: probability must be in [0, 1) and site must fit 32 bits")
     if o.probability == 0.0:
         return 0.0, None, o.site
     _state_check(name, state, device)
     return o.probability, state.data_ptr(), o.site
 
 
+# These calls take a few microseconds of host time on a small tensor, most of it here: the checks below read each property once,
+# build no message unless they fail, and take the current stream's pointer directly (0.2 us; through torch.cuda.Stream 3.6 us).
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _stream_on(name, device, stream):
     """Stream pointer of a call whose tensors are on `device`, which has to be the current device and the stream's."""
-    _require(device == torch.cuda.current_device() and (stream is None or stream.device_index == device),
-             f"{name}: tensors and stream must be on the current device")
-    return stream_ptr(stream)
+    if device != _current_device() or (stream is not None and stream.device_index != device):
+        _require(False, f"{name}: tensors and stream must be on the current device")
+    return _current_stream(device) if stream is None else stream.cuda_stream
 
 
 def _one_device(name, *tensors):
     """Device index of contiguous CUDA tensors of one dtype (None is skipped)."""
     first = tensors[0]
-    device, dtype = first.get_device(), first.dtype
+    device, dtype = first.get_device(), first.dtype      # -1: not a CUDA tensor
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.dtype == dtype and t.get_device() == device and t.is_contiguous()):
+        if t is not None and (t.dtype != dtype or t.get_device() != device or device < 0 or not t.is_contiguous()):
             _same_cuda_dtype(name, *[u for u in tensors if u is not None])
             _require(False, f"{name}: all tensors must be on one device")
     return device
@@ -531,11 +539,14 @@ def dropout_backward(grad_input, grad_output, state, stream=None, options: Dropo
 
 
 def _norm_shapes(name, x, weight, rows_like, vectors):
-    _require(x.dim() == 2 and weight.dim() == 1 and weight.shape[0] == x.shape[1], f"{name}: incompatible shapes")
+    shape, vector = x.shape, weight.shape
+    good = len(shape) == 2 and len(vector) == 1 and vector[0] == shape[1]
     for t in rows_like:
-        _require(t is None or t.shape == x.shape, f"{name}: incompatible shapes")
+        good = good and (t is None or t.shape == shape)
     for t in vectors:
-        _require(t is None or t.shape == weight.shape, f"{name}: incompatible shapes")
+        good = good and (t is None or t.shape == vector)
+    if not good:
+        _require(False, f"{name}: incompatible shapes")
 
 
 def layernorm_forward(output, input, weight, bias, epsilon, stream=None):
