@@ -244,12 +244,12 @@ layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __r
     }
 }
 
-#include "layernorm_rows.cuh"
 #include "layernorm_ring.cuh"
+#include "layernorm_loose.cuh"
 
 // How a call's rows are laid out. It follows from the sizes and the alignment alone, not from which operator is called, so that
 // the fused operators give the bits of their parts.
-enum class Form { kAny, kRows, kRing };
+enum class Form { kAny, kLoose, kRing };
 
 constexpr std::size_t kSmemPerSm = 227 * 1024;
 
@@ -257,27 +257,13 @@ constexpr std::size_t kSmemPerSm = 227 * 1024;
 std::size_t vectors_end(std::size_t hidden, std::size_t vectors) { return ring_kernels::kVectorsOffset + (vectors * hidden * sizeof(float) + 127) / 128 * 128; }
 
 // Rings take rows of which shared memory holds two stages of both tensors of the fused forward beside w and b, and of which a
-// CTA of the backward holds a row (14 k 16-bit or 8192 fp32 elements).
+// CTA of the backward holds a row (14 k 16-bit or 8192 fp32 elements). Others take the loose form up to 8192 elements.
 Form form_of(std::size_t hidden, std::size_t elem, bool vector) {
     if (vector && hidden * elem % 16 == 0)
         return hidden * elem / 16 <= ring_kernels::kTileVectors * ring_kernels::kBackwardThreads && vectors_end(hidden, 2) + 4 * hidden * elem <= kSmemPerSm ? Form::kRing : Form::kAny;
-    return hidden <= 16 * rows_kernels::kMaxTpr ? Form::kRows : Form::kAny;
-}
-
-// Rows of single elements: threads per row, row groups per CTA and (backward, 512 threads of up to 128 registers per SM) CTAs.
-struct RowsPlan {
-    int cpt, tpr, groups;
-    unsigned grid;
-};
-RowsPlan plan_rows(std::size_t rows, std::size_t hidden) {
-    RowsPlan p;
-    p.cpt = hidden <= 4 * rows_kernels::kMaxTpr ? 4 : 16;
-    p.tpr = static_cast<int>((hidden + p.cpt * 32 - 1) / (p.cpt * 32)) * 32;
-    p.groups = p.tpr < 256 ? 256 / p.tpr : 1;
-    const std::size_t at_once = static_cast<std::size_t>(p.groups) * (p.cpt == 4 ? 2 : 1), need = (rows + at_once - 1) / at_once;
-    const std::size_t cap = static_cast<std::size_t>(kNumSMs) * (512 / (p.groups * p.tpr));
-    p.grid = static_cast<unsigned>(need < cap ? need : cap);
-    return p;
+    const std::size_t row = hidden * elem + loose_kernels::kSlack + 128;      // the backward: two stages of three tensors beside w
+    return hidden <= loose_kernels::kMostColumns * loose_kernels::kBackwardThreads &&
+                   loose_kernels::kVectorsOffset + hidden * sizeof(float) + 6 * row + loose_kernels::kStatsBytes + 256 <= kSmemPerSm ? Form::kLoose : Form::kAny;
 }
 
 struct RingPlan {
@@ -343,6 +329,70 @@ RingPlan plan_backward_ring(std::size_t rows, std::size_t hidden, std::size_t el
     return p;
 }
 
+struct LoosePlan {
+    loose_kernels::LooseArgs args;
+    int columns, threads;      // columns per thread (backward)
+    unsigned grid;
+    std::size_t smem;
+};
+std::size_t loose_vectors_end(std::size_t hidden, std::size_t vectors) {
+    return loose_kernels::kVectorsOffset + (vectors * hidden * sizeof(float) + 127) / 128 * 128;
+}
+unsigned loose_tensor_bytes(std::size_t rows, std::size_t hidden, std::size_t elem) {
+    return static_cast<unsigned>((rows * hidden * elem + loose_kernels::kSlack + 127) / 128 * 128);
+}
+
+LoosePlan plan_forward_loose(std::size_t rows, std::size_t hidden, std::size_t elem, bool fused) {
+    LoosePlan p{};
+    auto& a = p.args;
+    a.warps_per_row = hidden <= 2048 ? 1 : hidden <= 4096 ? 2 : 4;
+    a.step_rows = static_cast<int>(hidden >= 1024 ? 1 : over(1024, hidden) < 32 ? over(1024, hidden) : 32);
+    a.data_offset = static_cast<unsigned>(loose_vectors_end(hidden, 2));
+    a.tensor_bytes = loose_tensor_bytes(a.step_rows, hidden, elem);
+    const std::size_t stage = (fused ? 2 : 1) * static_cast<std::size_t>(a.tensor_bytes), room = kSmemPerSm - a.data_offset;
+    std::size_t groups = loose_kernels::kForwardThreads / 32 / a.warps_per_row;
+    groups = at_most(at_most(groups, room / (2 * stage)), over(rows, static_cast<std::size_t>(kNumSMs) * a.step_rows));
+    if (a.warps_per_row > 1) groups = at_most(groups, 15);     // a named barrier each
+    a.groups = static_cast<int>(groups);
+    a.stages = static_cast<int>(at_most(room / groups / stage, ring_kernels::kMaxStages));
+    p.threads = a.groups * a.warps_per_row * 32;
+    p.smem = a.data_offset + groups * a.stages * stage;
+    p.grid = static_cast<unsigned>(at_most(over(rows, groups * a.step_rows), kNumSMs));
+    return p;
+}
+
+LoosePlan plan_backward_loose(std::size_t rows, std::size_t hidden, std::size_t elem) {
+    LoosePlan p{};
+    auto& a = p.args;
+    p.threads = hidden <= 2048 ? 256 : loose_kernels::kBackwardThreads;
+    p.columns = 1;
+    while (static_cast<std::size_t>(p.columns) * p.threads < hidden) p.columns *= 2;
+    const std::size_t ctas = loose_kernels::kBackwardThreads / p.threads;
+    a.groups = p.columns == 1 ? static_cast<int>(at_most(p.threads / hidden, loose_kernels::kMaxTileRows / 4)) : 1;
+    // Tiles of about 16 KB per tensor and CTA (more for one CTA), fewer rows when there are few: then every SM gets some.
+    std::size_t tile = at_most(16 * 1024 * (2 / ctas) / (hidden * elem), loose_kernels::kMaxTileRows);
+    tile = at_most(tile, over(rows, kNumSMs * ctas));
+    a.step_rows = static_cast<int>(tile < 1 ? 1 : tile);
+    const int warps = p.threads / 32;
+    a.warps_per_row = 1;
+    while (a.warps_per_row * a.step_rows * 2 <= warps && static_cast<std::size_t>(a.warps_per_row) * 64 < hidden) a.warps_per_row *= 2;
+    if (warps / a.warps_per_row > 8 && a.warps_per_row > 1) a.warps_per_row = warps / 8;   // 64 floats of sums per unit
+    a.data_offset = static_cast<unsigned>(loose_vectors_end(hidden, 1));
+    const std::size_t room = (kSmemPerSm + 1024) / ctas - 1024 - loose_kernels::kStatsBytes - a.data_offset;
+    std::size_t stage = 0;
+    for (;; --a.step_rows) {                                   // two stages at least, of one row if need be (form_of)
+        a.tensor_bytes = loose_tensor_bytes(a.step_rows, hidden, elem);
+        stage = 3 * static_cast<std::size_t>(a.tensor_bytes);     // room for a residual, whether there is one or not
+        if (a.step_rows == 1 || 2 * stage <= room) break;
+    }
+    a.stages = static_cast<int>(at_most(room / stage, ring_kernels::kMaxStages));
+    p.smem = a.data_offset + a.stages * stage;
+    const std::size_t joined = a.data_offset + 2 * hidden * sizeof(float);
+    if (p.smem < joined) p.smem = joined;
+    p.grid = static_cast<unsigned>(at_most(over(rows, a.step_rows), kNumSMs * ctas));
+    return p;
+}
+
 constexpr std::size_t kMaxSplits = 64;
 std::size_t any_splits(std::size_t rows) {
     const std::size_t n = (rows + 63) / 64;
@@ -371,7 +421,7 @@ std::size_t workspace_bytes(std::size_t rows, std::size_t hidden) {
         for (bool vector : {false, true}) {
             const Form form = form_of(hidden, elem, vector);
             const std::size_t n = form == Form::kRing ? plan_backward_ring(rows, hidden, elem).grid
-                                  : form == Form::kRows ? plan_rows(rows, hidden).grid : any_splits(rows);
+                                  : form == Form::kLoose ? plan_backward_loose(rows, hidden, elem).grid : any_splits(rows);
             if (n > parts) parts = n;
             if (form == Form::kAny) stats = rows * sizeof(float2);
         }
@@ -405,22 +455,19 @@ int launch_forward(void* y, void* sum, const void* x, const void* residual, cons
         auto either = [&](auto cpt) { return p.full ? launch(cpt, std::true_type{}) : launch(cpt, std::false_type{}); };
         return p.cpt == 1 ? either(Int<1>{}) : p.cpt == 2 ? either(Int<2>{}) : p.cpt == 4 ? either(Int<4>{}) : either(Int<8>{});
     }
-    if (form == Form::kRows) {
-        const RowsPlan p = plan_rows(rows, hidden);
-        auto launch = [&](auto cpt, auto r) {
-            auto kernel = rows_kernels::layernorm_forward_rows_kernel<T, cpt.value, r.value, FUSED>;
-            const int threads = p.groups * p.tpr;
-            const std::size_t at_once = static_cast<std::size_t>(p.groups) * r.value, need = (rows + at_once - 1) / at_once;
-            const std::size_t cap = static_cast<std::size_t>(kNumSMs) * resident_ctas_per_sm(reinterpret_cast<const void*>(kernel), threads, 0);
-            kernel<<<static_cast<unsigned>(need < cap ? need : cap), threads, 0, s>>>(
-                static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
-                static_cast<const T*>(w), static_cast<const T*>(b), static_cast<long long>(rows), static_cast<int>(hidden), epsilon,
-                p.tpr, args);
-            count_launch();
-            CGPT_LAUNCH_CHECK();
-            return CGPT_OK;
-        };
-        return p.cpt == 4 ? launch(Int<4>{}, Int<2>{}) : launch(Int<16>{}, Int<1>{});
+    if (form == Form::kLoose) {
+        LoosePlan p = plan_forward_loose(rows, hidden, sizeof(T), FUSED);
+        auto kernel = loose_kernels::layernorm_forward_loose_kernel<T, FUSED>;
+        static PerDeviceOnce once;
+        CGPT_TRY(allow_smem(kernel, &once));
+        p.args.status = tc_status_device_ptr();
+        if (p.args.status == nullptr) return CGPT_ERR_STATE;
+        kernel<<<p.grid, p.threads, p.smem, s>>>(
+            static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(w),
+            static_cast<const T*>(b), static_cast<long long>(rows), static_cast<int>(hidden), epsilon, p.args, args);
+        count_launch();
+        CGPT_LAUNCH_CHECK();
+        return CGPT_OK;
     }
     layernorm_forward_any_kernel<T, FUSED><<<any_grid(rows), kThreads, 0, s>>>(
         static_cast<T*>(y), static_cast<T*>(sum), static_cast<const T*>(x), static_cast<const T*>(residual),
@@ -464,20 +511,32 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
         if (p.cols == 1) return p.cpt == 1 ? either(Int<1>{}, Int<1>{}) : p.cpt == 2 ? either(Int<2>{}, Int<1>{}) : either(Int<4>{}, Int<1>{});
         return p.cols == 2 ? either(Int<4>{}, Int<2>{}) : either(Int<4>{}, Int<4>{});
     }
-    if (form == Form::kRows) {
-        const RowsPlan p = plan_rows(rows, hidden);
-        auto launch = [&](auto cpt, auto r) {
-            const std::size_t sums = static_cast<std::size_t>(p.groups) * 4 * r.value * 16 * sizeof(float);
-            const std::size_t parts = static_cast<std::size_t>(2) * cpt.value * p.tpr * sizeof(float);
-            rows_kernels::layernorm_backward_rows_kernel<T, cpt.value, r.value, FUSED><<<p.grid, p.groups * p.tpr, sums > parts ? sums : parts, s>>>(
+    if (form == Form::kLoose) {
+        const LoosePlan p = plan_backward_loose(rows, hidden, sizeof(T));
+        auto launch = [&](auto columns, auto threads) {
+            auto kernel = loose_kernels::layernorm_backward_loose_kernel<T, columns.value, threads.value, FUSED>;
+            static PerDeviceOnce once;
+            CGPT_TRY(allow_smem(kernel, &once, loose_kernels::kStatsBytes));
+            auto args_on_device = p.args;
+            args_on_device.status = tc_status_device_ptr();
+            if (args_on_device.status == nullptr) return CGPT_ERR_STATE;
+            kernel<<<p.grid, p.threads, p.smem, s>>>(
                 static_cast<T*>(dx), static_cast<T*>(din), partial, static_cast<const T*>(dy), static_cast<const T*>(x),
                 static_cast<const T*>(w), static_cast<const T*>(residual), static_cast<long long>(rows), static_cast<int>(hidden),
-                epsilon, p.tpr, args);
+                epsilon, args_on_device, args);
             count_launch();
             CGPT_LAUNCH_CHECK();
             return reduce(p.grid);
         };
-        return p.cpt == 4 ? launch(Int<4>{}, Int<2>{}) : launch(Int<16>{}, Int<1>{});
+        if (p.threads == 256) {
+            switch (p.columns) {
+                case 1: return launch(Int<1>{}, Int<256>{});
+                case 2: return launch(Int<2>{}, Int<256>{});
+                case 4: return launch(Int<4>{}, Int<256>{});
+                default: return launch(Int<8>{}, Int<256>{});
+            }
+        }
+        return p.columns == 8 ? launch(Int<8>{}, Int<512>{}) : launch(Int<16>{}, Int<512>{});
     }
     const std::size_t splits = any_splits(rows);
     float2* stats = reinterpret_cast<float2*>(partial + splits * 2 * hidden);

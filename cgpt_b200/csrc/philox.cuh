@@ -101,6 +101,15 @@ __device__ __forceinline__ float apply_one(float v, const Generator& gen, long l
     return ((i & 1) != 0 ? w : w << 16) >= a.threshold << 16 ? (SCALED ? __fmul_rn(v, a.scale) : v) : 0.f;
 }
 
+// A block's eight decisions as bits.
+__device__ __forceinline__ std::uint32_t kept_bits(const uint4& c, std::uint32_t threshold) {
+    const std::uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    std::uint32_t kept = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kept |= ((i & 1) != 0 ? w[i >> 1] : w[i >> 1] << 16) >= threshold << 16 ? 1u << i : 0u;
+    return kept;
+}
+
 // Decisions for four runs of 32 consecutive elements, one element of each run per lane: bit j of the result belongs to run j,
 // whose lane 0 has element start[j]. A run touches at most 5 generator blocks, so 8 lanes work out the blocks of one run and
 // hand the decisions round: one block per lane and 4 elements, not one per element.
@@ -111,11 +120,8 @@ __device__ __forceinline__ std::uint32_t keep_four_runs(const long long (&start)
 #pragma unroll
     for (int j = 1; j < 4; ++j)
         if ((lane >> 3) == j) mine = start[j];
-    const uint4 c = gen.block(static_cast<std::uint32_t>(mine >> 3) + (lane & 7));
-    const std::uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    std::uint32_t kept = 0, out = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) kept |= (((i & 1) != 0 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu) >= threshold ? 1u : 0u) << i;
+    const std::uint32_t kept = kept_bits(gen.block(static_cast<std::uint32_t>(mine >> 3) + (lane & 7)), threshold);
+    std::uint32_t out = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int at = static_cast<int>(start[j] & 7) + lane;      // element of lane `lane`, counted from the run's first block
