@@ -110,8 +110,9 @@ struct WarpSums {
             for (int i = 0; i < kCount; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
         }
     }
-    // Every lane gets every total.
+    // Every lane gets every total (and has it already where nothing was halved).
     static __device__ __forceinline__ void broadcast(float (&v)[NV]) {
+        if constexpr (NV % 2 != 0) return;
         float t[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) t[i] = __shfl_sync(0xffffffffu, v[i % kCount], holder_of(i));

@@ -298,28 +298,28 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     const unsigned lane_bytes = lane_row * ring.row_bytes + vec0 * 16, next_row = per_warp * ring.row_bytes;
     const int next_elements = ra.groups * hidden;
     __syncthreads();
-    Pair wv[COLS][NP], aw[COLS][NP], ab[COLS][NP];
+    Pair wv[NP] = {}, aw[COLS][NP], ab[COLS][NP];            // w of the thread's columns, if they are few: else read where needed
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) {
-        const int vec = column + c * blockDim.x;
+    for (int c = 0; c < COLS; ++c)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) wv[c][i] = aw[c][i] = ab[c][i] = 0;
-        if (vec < ra.vectors) read_pairs<NP>(wv[c], ws, vec, ra.vectors);
-    }
+        for (int i = 0; i < NP; ++i) aw[c][i] = ab[c][i] = 0;
+    if (COLS == 1) read_pairs<NP>(wv, ws, column, ra.vectors);
 
     int buffer = 0;
     for (long long row0 = first; row0 < rows; row0 += step, buffer ^= 1) {
         const int tile_rows = rows - row0 < ra.step_rows ? static_cast<int>(rows - row0) : ra.step_rows;
         const long long e0 = (row0 + row_group) * hidden + column * VEC;       // the thread's first element in the column phase
+        const bool whole = tile_rows == ra.step_rows;
         // The residual is needed last: on its way past the ring while the row sums are taken.
         uint4 rp[RC][COLS];
         if (residual != nullptr && works) {
+            const T* from = residual + e0;
 #pragma unroll
-            for (int k = 0; k < RC; ++k)
+            for (int k = 0; k < RC; ++k, from += next_elements)
 #pragma unroll
                 for (int c = 0; c < COLS; ++c)
-                    if (k * ra.groups + row_group < tile_rows && (COLS == 1 || column + c * blockDim.x < ra.vectors))
-                        rp[k][c] = __ldcs(reinterpret_cast<const uint4*>(residual + e0 + k * next_elements + c * blockDim.x * VEC));
+                    if ((whole || k * ra.groups + row_group < tile_rows) && (COLS == 1 || column + c * blockDim.x < ra.vectors))
+                        rp[k][c] = __ldcs(reinterpret_cast<const uint4*>(from + c * blockDim.x * VEC));
         }
         const unsigned char* stage = ring.wait();
         // ---- rows: four sums each
@@ -402,40 +402,44 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
         if (threadIdx.x == 0 && row0 != first)
             ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, none, row0 + (ring.stages - 1) * step, ra.step_rows, rows, hidden);
         // ---- columns
-        if (works) {
+        auto columns = [&](auto all_rows) {
             const unsigned char* at = stage + column_bytes;
+            const ulonglong2(*st)[2] = stats[buffer] + row_group;
+            long long e = e0;
 #pragma unroll
-            for (int k = 0; k < RC; ++k) {
-                const int row = k * ra.groups + row_group;
-                if (row < tile_rows) {
-                    const ulonglong2 st = stats[buffer][row][0], cs = stats[buffer][row][1];
+            for (int k = 0; k < RC; ++k, at += next_rows, st += ra.groups, e += next_elements) {
+                if (all_rows.value || k * ra.groups + row_group < tile_rows) {
+                    const ulonglong2 norm = st[0][0], cs = st[0][1];
 #pragma unroll
                     for (int c = 0; c < COLS; ++c) {
                         if (COLS == 1 || column + c * blockDim.x < ra.vectors) {
-                            const unsigned char* here = at + k * next_rows + c * blockDim.x * 16;
-                            const long long e = e0 + k * next_elements + c * blockDim.x * VEC;
                             Pair v[NP], g[NP], out[NP];
-                            to_pairs<T>(v, *reinterpret_cast<const uint4*>(here));
-                            to_pairs<T>(g, *reinterpret_cast<const uint4*>(here + ring.tensor_bytes));
+                            to_pairs<T>(v, *reinterpret_cast<const uint4*>(at + c * blockDim.x * 16));
+                            to_pairs<T>(g, *reinterpret_cast<const uint4*>(at + ring.tensor_bytes + c * blockDim.x * 16));
 #pragma unroll
                             for (int i = 0; i < NP; ++i) out[i] = 0;
                             if (residual != nullptr) to_pairs<T>(out, rp[k][c]);
+                            if constexpr (COLS > 1) read_pairs<NP>(wv, ws, column + c * blockDim.x, ra.vectors);
 #pragma unroll
                             for (int i = 0; i < NP; ++i) {
-                                const Pair xh = mul2(add2(v[i], st.x), st.y);
-                                out[i] = fma2(st.y, fma2(xh, cs.y, fma2(g[i], wv[c][i], cs.x)), out[i]);
+                                const Pair xh = mul2(add2(v[i], norm.x), norm.y);
+                                out[i] = fma2(norm.y, fma2(xh, cs.y, fma2(g[i], wv[i], cs.x)), out[i]);
                                 aw[c][i] = fma2(g[i], xh, aw[c][i]);
                                 ab[c][i] = add2(ab[c][i], g[i]);
                             }
-                            *reinterpret_cast<uint4*>(dx + e) = to_raw<T>(out);
+                            *reinterpret_cast<uint4*>(dx + e + c * blockDim.x * VEC) = to_raw<T>(out);
                             if constexpr (FUSED) {
-                                if (args.threshold != 0) drop_pairs<NP>(out, gen, e, args);
-                                *reinterpret_cast<uint4*>(din + e) = to_raw<T>(out);
+                                if (args.threshold != 0) drop_pairs<NP>(out, gen, e + c * blockDim.x * VEC, args);
+                                *reinterpret_cast<uint4*>(din + e + c * blockDim.x * VEC) = to_raw<T>(out);
                             }
                         }
                     }
                 }
             }
+        };
+        if (works) {
+            if (whole) columns(std::true_type{});
+            else columns(std::false_type{});
         }
         ring.next();
     }
