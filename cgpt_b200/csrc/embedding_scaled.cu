@@ -16,6 +16,7 @@
 //
 // Memory-bound without dropout: backward reads dout once and writes the table once; the sort moves 16 bytes per token and pass.
 #include <algorithm>
+#include <atomic>
 
 #include <cooperative_groups.h>
 
@@ -700,35 +701,61 @@ int launch_sum(void* dw, const void* dout, GradArgs g, const DropoutArgs& args, 
     return CGPT_OK;
 }
 
-constexpr std::size_t kClusterTokens = std::size_t{kMostKeys} * kMaxCluster * kClusterThreads;
+// Clusters of the sort by keys per thread (1, 2, kMostKeys).
+void (*const kClusterKernels[3])(ClusterSort) = {sort_cluster_kernel<1>, sort_cluster_kernel<2>, sort_cluster_kernel<kMostKeys>};
+constexpr std::size_t kClusterSmem[3] = {sizeof(ClusterSmem<1>), sizeof(ClusterSmem<2>), sizeof(ClusterSmem<kMostKeys>)};
 
-// One launch of one cluster, up to kClusterTokens tokens.
-int launch_cluster_sort(const ClusterSort& p, cudaStream_t s) {
-    int ctas = 1;
-    while (ctas < kMaxCluster && ctas * kClusterThreads < p.n) ctas *= 2;
-    const int keys = (p.n + ctas * kClusterThreads - 1) / (ctas * kClusterThreads);
-    const int size = keys == 1 ? 0 : keys == 2 ? 1 : 2;
-    void (*const kernels[3])(ClusterSort) = {sort_cluster_kernel<1>, sort_cluster_kernel<2>, sort_cluster_kernel<kMostKeys>};
-    constexpr std::size_t smem[3] = {sizeof(ClusterSmem<1>), sizeof(ClusterSmem<2>), sizeof(ClusterSmem<kMostKeys>)};
-    auto kernel = kernels[size];
+int cluster_config(cudaLaunchConfig_t* config, cudaLaunchAttribute* attribute, int size, int ctas, cudaStream_t s) {
     static PerDeviceOnce once[3];
     if (once[size].needed()) {
-        CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-        CGPT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem[size])));
+        CGPT_CUDA_TRY(cudaFuncSetAttribute(kClusterKernels[size], cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CGPT_CUDA_TRY(cudaFuncSetAttribute(kClusterKernels[size], cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kClusterSmem[size])));
         once[size].done();
     }
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(p.clear != nullptr ? 128 / ctas * ctas : ctas);   // clusters of 16 that fit on the SMs at a time: 8
-    config.blockDim = dim3(kClusterThreads);
-    config.dynamicSmemBytes = smem[size];
-    config.stream = s;
+    *config = cudaLaunchConfig_t{};
+    config->gridDim = dim3(ctas);
+    config->blockDim = dim3(kClusterThreads);
+    config->dynamicSmemBytes = kClusterSmem[size];
+    config->stream = s;
+    attribute->id = cudaLaunchAttributeClusterDimension;
+    attribute->val.clusterDim.x = ctas;
+    attribute->val.clusterDim.y = attribute->val.clusterDim.z = 1;
+    config->attrs = attribute;
+    config->numAttrs = 1;
+    return CGPT_OK;
+}
+
+// CTAs of the largest cluster that the current device places: 16, or the 8 that every device has to, where a part of the GPU is
+// not ours. Asked once per device.
+int most_cluster_ctas(int* ctas) {
+    static std::atomic<int> known[64];
+    int device = 0;
+    CGPT_CUDA_TRY(cudaGetDevice(&device));
+    if (device < 0 || device >= 64) return CGPT_ERR_UNSUPPORTED;
+    *ctas = known[device].load(std::memory_order_relaxed);
+    if (*ctas == 0) {
+        cudaLaunchConfig_t config;
+        cudaLaunchAttribute attribute;
+        CGPT_TRY(cluster_config(&config, &attribute, 2, kMaxCluster, nullptr));
+        int n = 0;
+        const bool fits = cudaOccupancyMaxActiveClusters(&n, kClusterKernels[2], &config) == cudaSuccess && n > 0;
+        cudaGetLastError();
+        *ctas = fits ? kMaxCluster : 8;
+        known[device].store(*ctas, std::memory_order_relaxed);
+    }
+    return CGPT_OK;
+}
+
+// One launch: a cluster that sorts, others that clear. p.n <= most * kClusterThreads * kMostKeys.
+int launch_cluster_sort(const ClusterSort& p, int most, cudaStream_t s) {
+    int ctas = 1;
+    while (ctas < most && ctas * kClusterThreads < p.n) ctas *= 2;
+    const int keys = (p.n + ctas * kClusterThreads - 1) / (ctas * kClusterThreads), size = keys == 1 ? 0 : keys == 2 ? 1 : 2;
+    cudaLaunchConfig_t config;
     cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = ctas;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    CGPT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+    CGPT_TRY(cluster_config(&config, &attribute, size, ctas, s));
+    if (p.clear != nullptr) config.gridDim = dim3(128 / ctas * ctas);   // clusters of 16 that fit on the SMs at a time: 8
+    CGPT_CUDA_TRY(cudaLaunchKernelEx(&config, kClusterKernels[size], p));
     count_launch();
     return CGPT_OK;
 }
@@ -789,18 +816,21 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
     const int bits = bit_length(vocab);   // keys are in [0, vocab]
     const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     const int digit_bits = (bits + passes - 1) / passes;
+    int most = 0;
+    CGPT_TRY(most_cluster_ctas(&most));
+    const bool one_cluster = tokens <= static_cast<std::size_t>(most) * kClusterThreads * kMostKeys;
     const std::size_t table_bytes = vocab * hidden * dtype_size(dtype);
     ClusterSort c{};
     // The table starts on an element, the vectors that clear it on 16 bytes: the few bytes before go with a small memset.
     const std::size_t lead = std::min<std::size_t>((16 - (reinterpret_cast<std::uintptr_t>(grad_weight) & 15)) & 15, table_bytes);
     if (!accumulate) {
-        if (lead != 0 || tokens > kClusterTokens) CGPT_CUDA_TRY(cudaMemsetAsync(grad_weight, 0, tokens > kClusterTokens ? table_bytes : lead, s));
+        if (lead != 0 || !one_cluster) CGPT_CUDA_TRY(cudaMemsetAsync(grad_weight, 0, one_cluster ? lead : table_bytes, s));
         c.clear = reinterpret_cast<uint4*>(static_cast<unsigned char*>(grad_weight) + lead);
         c.clear_vectors = static_cast<long long>((table_bytes - lead) / 16);
         c.clear_tail = static_cast<int>((table_bytes - lead) % 16);
     }
     c.ids = ids;
-    const int last = tokens <= kClusterTokens ? 0 : (passes - 1) & 1;   // which buffers the sorted tokens end up in
+    const int last = one_cluster ? 0 : (passes - 1) & 1;   // which buffers the sorted tokens end up in
     c.keys = words(at.keys[last]);
     c.vals = words(at.vals[last]);
     c.crossing = words(at.crossing);
@@ -809,8 +839,8 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
     c.passes = passes;
     c.vocab = static_cast<std::uint32_t>(vocab);
     c.skip_id = padding_id;
-    if (tokens <= kClusterTokens) {
-        CGPT_TRY(launch_cluster_sort(c, s));
+    if (one_cluster) {
+        CGPT_TRY(launch_cluster_sort(c, most, s));
     } else {
         SortPass p{};
         p.counts = words(at.counts);

@@ -145,7 +145,8 @@ def test_dropout_beyond_32_bit_offsets(ops, state):
 # --------------------------------------------------------------------------------------------------------- layer norm
 # rows of one element, below a vector, at and around every change of layout, and beyond what registers hold
 SHAPES = [(1, 1), (5, 2), (3, 7), (1, 8), (2, 64), (9, 100), (33, 250), (64, 256), (7, 257), (130, 512), (65, 688), (31, 1000), (17, 1001),
-          (40, 1024), (12, 1032), (11, 2048), (300, 2056), (6, 4096), (5, 5000), (4, 8192), (3, 8200), (3, 16384), (3, 16385), (2, 33000), (2, 70001)]
+          (37, 712), (40, 1024), (12, 1032), (9, 1537), (11, 2048), (300, 2056), (6, 4096), (7, 4099), (5, 5000), (6, 6008), (4, 8191), (4, 8192), (3, 8200), (2, 12008),
+          (3, 14016), (3, 16384), (3, 16385), (2, 33000), (2, 70001)]
 
 
 def norm_inputs(rows, hidden, dt, seed=0):
@@ -186,7 +187,7 @@ def test_layernorm(ops, dt, rows, hidden):
 def test_layernorm_misaligned_tensors(ops, rows, hidden):
     dt = "bf16"
     arrays = [host(t) for t in norm_inputs(rows, hidden, dt)]
-    x, w, b, dy, res = (shifted(a, dt, 1) for a in arrays)
+    x, w, b, dy, res = (shifted(a, dt, k) for a, k in zip(arrays, (1, 2, 3, 5, 6)))
     X, W, B, DY, RES = arrays
     y, dx, dw, db = (Guarded(s, dt, 1) for s in (x.shape, x.shape, w.shape, w.shape))
     ops.layernorm_forward(y.t, x, w, b, 1e-5)
@@ -200,7 +201,7 @@ def test_layernorm_misaligned_tensors(ops, rows, hidden):
         close(got.check(), v, P.rounding(v, torch.bfloat16) + 2 * e, what)
 
 
-@pytest.mark.parametrize("rows,hidden", [(3000, 256), (2500, 1024), (1500, 2048), (700, 4096), (600, 1001), (3000, 24), (1, 4096), (20000, 8)])
+@pytest.mark.parametrize("rows,hidden", [(3000, 256), (2500, 1024), (1500, 2048), (700, 4096), (400, 8192), (600, 1001), (900, 2303), (300, 7001), (5000, 130), (5000, 61), (9001, 3), (3000, 24), (1, 4096), (20000, 8)])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_layernorm_many_rows_repeat_bit_for_bit(ops, dt, rows, hidden):
     x, w, _, dy, _ = norm_inputs(rows, hidden, dt)
@@ -311,8 +312,9 @@ def test_fused_equals_its_parts(ops, state, dt, rows, hidden):
             assert torch.equal(buffer, dr.t)
 
 
-def test_fused_in_place_sum_and_no_dropout(ops, state):
-    x, w, b, _, res = norm_inputs(37, 512, "f16")
+@pytest.mark.parametrize("hidden", [512, 511, 3000, 2999, 20000])
+def test_fused_in_place_sum_and_no_dropout(ops, state, hidden):
+    x, w, b, _, res = norm_inputs(1200, hidden, "f16")
     o = ops.DropoutOptions(0.4, 1)
     y, total = torch.empty_like(x), torch.empty_like(x)
     ops.dropout_add_layernorm_forward(y, total, x, res, w, b, 1e-5, state, options=o)
