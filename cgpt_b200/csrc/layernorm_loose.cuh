@@ -81,6 +81,13 @@ struct Ring {
     __device__ __forceinline__ void next() {
         if (++stage == stages) { stage = 0; parity ^= 1u; }
     }
+    // Before the CTA leaves: copies that a failed wait gave up on get time to land while the memory is still its own.
+    __device__ __forceinline__ void leave() const {
+        if (failed) {
+            const unsigned long long t0 = sm100::globaltimer_ns();
+            while (sm100::globaltimer_ns() - t0 < 200000ull) { }
+        }
+    }
 };
 
 // Orders this thread's stores to a stage before the copies that refill it after the next barrier.
@@ -219,6 +226,7 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
         if (tid == 0) ring.fill(ring.stage, x, second, none, row0 + ring.stages * step, la.step_rows, rows, hidden);
         ring.next();
     }
+    ring.leave();
 }
 
 // Tiles of rows in two phases, as ring_kernels: a warp group per row for the sums, then a thread per column. K columns per thread,
@@ -333,6 +341,7 @@ layernorm_backward_loose_kernel(T* dx, T* din, float* __restrict__ partial, cons
         }
         ring.next();
     }
+    ring.leave();
     // One partial row of dw and of db per CTA: its row groups add up one after the other, in the memory of the ring, whose copies
     // have all been waited for.
     float* out_w = partial + static_cast<long long>(blockIdx.x) * 2 * hidden;

@@ -63,6 +63,13 @@ struct Ring {
     __device__ __forceinline__ void next() {
         if (++stage == stages) { stage = 0; parity ^= 1u; }
     }
+    // Before the CTA leaves: copies that a failed wait gave up on get time to land while the memory is still its own.
+    __device__ __forceinline__ void leave() const {
+        if (failed) {
+            const unsigned long long t0 = sm100::globaltimer_ns();
+            while (sm100::globaltimer_ns() - t0 < 200000ull) { }
+        }
+    }
 };
 
 // Layout of a launch: vectors per row, lanes per row (fewer than 32 where a warp holds several rows), warps per row, rows a group
@@ -252,6 +259,7 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
             }
         }
     }
+    ring.leave();
 }
 
 // CPT: vectors per lane in the row phase (FULL: exactly the row's). COLS: vectors per thread and row in the column phase.
@@ -443,6 +451,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
         }
         ring.next();
     }
+    ring.leave();
 
     // One partial row of dw and of db per CTA: its row groups add up one after the other, in the memory of the ring, whose copies
     // have all been waited for.
