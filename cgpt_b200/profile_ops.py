@@ -3,7 +3,8 @@ than L2 but a few hundred MB at most, so that `ncu -k regex:<kernel>` captures o
 Ops: gemm_fwd, gemm_dx, gemm_dw, linear_sum (output + down projection + residual as one product), attention_fwd,
 attention_bwd, rmsnorm_bwd, rmsnorm_dual_fwd, rmsnorm_dual_bwd (both norms of one input in one pass), swiglu_bwd, rope_bwd, embedding_bwd, adamw,
 cross_entropy, cce (one 8192-row chunk of the cut cross-entropy at hidden 1024, vocabulary 32000; --cce-form 1|2|3),
-qknorm_fwd, qknorm_bwd.
+qknorm_fwd, qknorm_bwd, and the pre-norm block's layernorm_fwd, layernorm_bwd, dropout (with residual), dropout_add_layernorm_fwd,
+dropout_add_layernorm_bwd, scaled_embedding_fwd, scaled_embedding_bwd (dropout 0.1; --hidden sets the width).
 Prints the CUDA-event time per launch (taken without a profiler attached it is the number to quote)."""
 from __future__ import annotations
 
@@ -27,6 +28,37 @@ def _run(fn, iters):
     return e0.elapsed_time(e1) / iters
 
 
+PRENORM = ("layernorm_fwd", "layernorm_bwd", "dropout", "dropout_add_layernorm_fwd", "dropout_add_layernorm_bwd", "scaled_embedding_fwd",
+           "scaled_embedding_bwd")
+
+
+def _prenorm(a, h, T) -> None:
+    """The pre-norm block's operators on T rows; bytes are those of the operands, each read or written once."""
+    d, V = a.hidden, 32000
+    drop, state = ops.DropoutOptions(0.1, 0), ops.make_dropout_state(1)
+    w, b, dw, db = (torch.ones(d, device="cuda").half() for _ in range(4))
+    if a.op.startswith("scaled_embedding"):
+        ids = (V ** torch.rand(T, device="cuda", dtype=torch.float64)).long().sub_(1).clamp_(0, V - 1).int()   # frequencies fall as 1 / rank
+        table, x, o = h(V, d), h(T, d), ops.ScaledEmbeddingOptions(d ** 0.5, dropout=drop)
+        if a.op.endswith("fwd"):
+            fn, nbytes = lambda: ops.scaled_embedding_forward(x, ids, T, table, state, options=o), (T + ids.unique().numel()) * d * 2
+        else:
+            fn, nbytes = lambda: ops.scaled_embedding_backward(table, x, ids, T, state, options=o), (T + V) * d * 2
+    else:
+        x, y, r, s = h(T, d), h(T, d), h(T, d), h(T, d)
+        z = torch.empty_like(x)
+        fn, tensors = {
+            "layernorm_fwd": (lambda: ops.layernorm_forward(y, x, w, b, 1e-5), 2),
+            "layernorm_bwd": (lambda: ops.layernorm_backward(y, dw, db, r, x, w, 1e-5), 3),
+            "dropout": (lambda: ops.dropout_forward(y, x, state, options=drop, residual=r), 3),
+            "dropout_add_layernorm_fwd": (lambda: ops.dropout_add_layernorm_forward(y, s, x, r, w, b, 1e-5, state, options=drop), 4),
+            "dropout_add_layernorm_bwd": (lambda: ops.dropout_add_layernorm_backward(y, z, dw, db, r, s, x, w, 1e-5, state, options=drop), 5),
+        }[a.op]
+        nbytes = tensors * T * d * 2
+    ms = _run(fn, a.iters)
+    print(f"{a.op} {T}x{d}: {ms * 1e3:.1f} us, {nbytes / ms / 1e6:.0f} GB/s algorithmic")
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("op")
@@ -35,6 +67,7 @@ def main() -> None:
                     help="attention ops: 8/2 heads of 128 (the 104m layer) or 12/4 heads of 64")
     ap.add_argument("--cce-form", type=int, default=0, help="cce: 0 default, 1 row kernel, 2 tile statistics, 3 recompute")
     ap.add_argument("--rows", type=int, default=8192, help="cce: rows (8192 is one chunk)")
+    ap.add_argument("--hidden", type=int, default=1024, help="layer norm, dropout and scaled embedding: elements per row")
     ap.add_argument("--cce-chunk", type=int, default=0, help="cce: rows per chunk (0 = the library's choice)")
     a = ap.parse_args()
     h = lambda *s: torch.randn(*s, device="cuda").half()
@@ -152,6 +185,8 @@ def main() -> None:
             nbytes = 3 * (q.numel() + k.numel()) * 2
         ms = _run(fn, a.iters)
         print(f"{a.op} B{B} S{S} {Hq}/{Hkv} D{D}: {ms * 1e3:.1f} us, {nbytes / ms / 1e6:.0f} GB/s algorithmic")
+    elif a.op in PRENORM:
+        _prenorm(a, h, T)
     else:
         raise SystemExit(f"unknown op {a.op}")
 
