@@ -580,7 +580,7 @@ constexpr int kJoinThreads = 256;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kJoinThreads)
 scaled_embedding_join_kernel(T* dw, const GradArgs g) {
-    __shared__ float tile[kJoinThreads / 32][32 * VEC];
+    __shared__ __align__(16) float tile[kJoinThreads / 32][32 * VEC];
     const int lane = threadIdx.x & 31, pl = threadIdx.x >> 5;
     wait_for_previous();
     const unsigned column_tiles = static_cast<unsigned>((g.hidden + 32 * VEC - 1) / (32 * VEC)), runs = *g.crossing;
@@ -607,6 +607,187 @@ scaled_embedding_join_kernel(T* dw, const GradArgs g) {
 #pragma unroll
             for (int r = 0; r < kJoinThreads / 32; ++r) add_floats<VEC>(t, &tile[r][lane * VEC]);
             write_row<T, VEC>(dw + static_cast<long long>(id) * g.hidden + col, t, g.scale, g.accumulate);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- few tokens
+// One launch for few tokens and a small table: sort, sums and joins would be three, of a few microseconds of latency each. A
+// CTA owns every gridDim.x-th row of the table (frequent ids are often neighbours) and a tile of columns. It picks the tokens of
+// its rows out of all ids, in token order, zeroes its rows that have none, and adds up the others, a warp per row; rows with
+// more than kFewOfRow tokens are shared out to all warps afterwards, each taking a part of the list. The order of every sum
+// follows from the ids alone.
+// The rule (takes_few) by what was measured on both sides, us for one launch against the sort's three, dropout 0.1:
+// vectors, 4 MB table: 1 token f32 1024 wide 8 | 12; 128 tokens f32 256 wide 10 | 14; 512 tokens bf16 1024 wide 17 | 19, f32
+// 768 wide 16 | 21; 1024 tokens 22 | 18; 512 tokens and 8 MB 20 | 19; 32 MB 34 | 21 (rows cleared one by one).
+// Single elements, 513 wide: 1024 tokens f32 4 MB 23 | 33, bf16 16 MB 27 | 33; 1 token, 16 MB 12 | 16. Vectors do best with
+// a warp's width of columns per CTA (four: 33 instead of 27 for 1024 wide), single elements with four.
+constexpr int kFewTokens = 1024, kFewOfRow = 32, kFewThreads = 512, kFewWarps = kFewThreads / 32;
+constexpr unsigned kFewRows = 16384;     // rows of a CTA at most (a bit each)
+
+struct FewArgs {
+    const std::uint32_t* ids;
+    int tokens, hidden, tile, accumulate;        // tile: columns per CTA
+    std::uint32_t vocab, skip_id;
+    float scale;
+};
+
+// Adds the rows of `count` listed tokens to acc, kInFlight at a time. Every lane of the warp takes part, whether it has columns
+// (`in`) or not: single elements share their decisions.
+template <typename T, int VEC, typename Generator>
+__device__ __forceinline__ void add_rows(float (&acc)[VEC], const T* dout, const std::uint32_t* list, int count, int hidden, int c, bool in, const Generator& gen,
+                                         const DropoutArgs& args) {
+    using Raw = typename RawVec<sizeof(T) * VEC>::type;
+    for (int k = 0; k < count; k += kInFlight) {
+        Raw rows[kInFlight];
+        long long e[kInFlight];
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+            e[u] = static_cast<long long>(list[k + u < count ? k + u : k]) * hidden + c;      // past the end: the first one again, not added
+            rows[u] = *reinterpret_cast<const Raw*>(dout + (in ? e[u] : 0));
+        }
+        std::uint32_t kept = 15u;
+        if constexpr (VEC == 1) {
+            if (args.threshold != 0) {
+                long long start[kInFlight];
+#pragma unroll
+                for (int u = 0; u < kInFlight; ++u) start[u] = e[u] - static_cast<int>(threadIdx.x & 31);
+                kept = keep_four_runs(start, gen, args.threshold);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+            if (k + u < count) {
+                if constexpr (VEC > 1) {
+                    Pair v[VEC / 2];
+                    to_pairs<T>(v, rows[u]);
+                    if (args.threshold != 0) drop_pairs<VEC / 2, false>(v, gen, e[u], args);
+#pragma unroll
+                    for (int i = 0; i < VEC / 2; ++i) {
+                        const float2 f = both(v[i]);
+                        acc[2 * i] += f.x;
+                        acc[2 * i + 1] += f.y;
+                    }
+                } else if ((kept >> u) & 1u) {
+                    acc[0] += to_f32<T>(*reinterpret_cast<const T*>(&rows[u]));
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kFewThreads)
+scaled_embedding_few_kernel(T* dw, const T* __restrict__ dout, const FewArgs f, const DropoutArgs args) {
+    __shared__ std::uint32_t token[kFewTokens], row_of[kFewTokens];      // the tokens of this CTA's rows, in token order
+    __shared__ std::uint32_t present[kFewRows / 32];
+    __shared__ std::uint32_t heads[kFewTokens];                         // list positions at which a row is met first
+    __shared__ std::uint32_t few[kFewWarps][kFewOfRow];                  // per warp: the tokens of the row it adds up
+    __shared__ int in_warp[kFewWarps], listed, rows_listed;
+    __shared__ __align__(16) float part[kFewWarps][32 * VEC];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const std::uint32_t shares = gridDim.x, rows = (f.vocab - blockIdx.x + shares - 1) / shares;     // row r of the CTA: r * shares + blockIdx.x
+    const int c_begin = blockIdx.y * f.tile, c_end = c_begin + f.tile < f.hidden ? c_begin + f.tile : f.hidden;
+    const HoistedPhilox gen(args);
+    for (unsigned i = threadIdx.x; i < (rows + 31) / 32; i += kFewThreads) present[i] = 0;
+    if (threadIdx.x == 0) rows_listed = 0;
+    __syncthreads();
+    int so_far = 0;
+    for (int t0 = 0; t0 < f.tokens; t0 += kFewThreads) {
+        const int t = t0 + threadIdx.x;
+        const std::uint32_t id = t < f.tokens ? f.ids[t] : 0xffffffffu;
+        const std::uint32_t row = id / shares;
+        const bool mine = t < f.tokens && id < f.vocab && id != f.skip_id && id - row * shares == blockIdx.x;
+        const unsigned votes = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) in_warp[warp] = __popc(votes);
+        __syncthreads();
+        int at = so_far + __popc(votes & ((1u << lane) - 1u)), all = 0;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) {
+            at += w < warp ? in_warp[w] : 0;
+            all += in_warp[w];
+        }
+        if (mine) {
+            token[at] = t;
+            row_of[at] = row;
+            atomicOr(&present[row >> 5], 1u << (row & 31));
+        }
+        so_far += all;
+        __syncthreads();
+    }
+    const int n = so_far;
+    if (!f.accumulate) {
+        const float zero[VEC] = {};
+        for (unsigned word = warp; word < (rows + 31) / 32; word += kFewWarps) {
+            unsigned todo = ~present[word];
+            if (rows - word * 32 < 32) todo &= (1u << (rows - word * 32)) - 1u;
+            while (todo != 0) {
+                T* to = dw + (static_cast<long long>(word * 32 + __ffs(todo) - 1) * shares + blockIdx.x) * f.hidden;
+                todo &= todo - 1;
+                for (int c = c_begin + lane * VEC; c < c_end; c += 32 * VEC) store_vec<T, VEC>(to + c, zero);
+            }
+        }
+    }
+    for (int i = threadIdx.x; i < n; i += kFewThreads) {
+        bool first = true;
+        for (int j = 0; j < i && first; ++j) first = row_of[j] != row_of[i];
+        if (first) heads[atomicAdd(&rows_listed, 1)] = i;                // their order changes no result
+    }
+    __syncthreads();
+    for (int h = warp; h < rows_listed; h += kFewWarps) {                // a warp per row of up to kFewOfRow tokens
+        const int first = heads[h];
+        const std::uint32_t row = row_of[first];
+        int count = 0;
+        for (int i0 = first; i0 < n; i0 += 32) {
+            const bool same = i0 + lane < n && row_of[i0 + lane] == row;
+            const unsigned votes = __ballot_sync(0xffffffffu, same);
+            const int at = count + __popc(votes & ((1u << lane) - 1u));
+            if (same && at < kFewOfRow) few[warp][at] = token[i0 + lane];
+            count += __popc(votes);
+        }
+        __syncwarp();
+        if (count <= kFewOfRow) {
+            for (int c0 = c_begin; c0 < c_end; c0 += 32 * VEC) {
+                const int c = c0 + lane * VEC;
+                float acc[VEC] = {};
+                add_rows<T, VEC>(acc, dout, few[warp], count, f.hidden, c, c < c_end, gen, args);
+                if (c < c_end) write_row<T, VEC>(dw + (static_cast<long long>(row) * shares + blockIdx.x) * f.hidden + c, acc, f.scale, f.accumulate);
+            }
+        }
+        __syncwarp();
+    }
+    if (n <= kFewOfRow) return;
+    // Rows of more tokens: every warp adds those in its part of the list, then the parts are added in order.
+    const int share = (n + kFewWarps - 1) / kFewWarps, begin = warp * share, end = begin + share < n ? begin + share : n;
+    for (int h = 0; h < rows_listed; ++h) {
+        const int first = heads[h];
+        const std::uint32_t row = row_of[first];
+        int count = 0;
+        for (int i = first + threadIdx.x; i < n; i += kFewThreads) count += row_of[i] == row;
+        if (__syncthreads_count(count != 0) <= kFewOfRow) {              // at most one token a thread is counted: look closer
+            int total = 0;
+            for (int i0 = first; i0 < n; i0 += 32) total += __popc(__ballot_sync(0xffffffffu, i0 + lane < n && row_of[i0 + lane] == row));
+            if (total <= kFewOfRow) continue;                            // the same in every warp
+        }
+        for (int c0 = c_begin; c0 < c_end; c0 += 32 * VEC) {
+            const int c = c0 + lane * VEC;
+            float acc[VEC] = {};
+            for (int i0 = begin; i0 < end; i0 += 32) {
+                const bool same = i0 + lane < end && row_of[i0 + lane] == row;
+                const unsigned votes = __ballot_sync(0xffffffffu, same);
+                __syncwarp();
+                if (same) few[warp][__popc(votes & ((1u << lane) - 1u))] = token[i0 + lane];
+                __syncwarp();
+                add_rows<T, VEC>(acc, dout, few[warp], __popc(votes), f.hidden, c, c < c_end, gen, args);
+            }
+            put_floats<VEC>(&part[warp][lane * VEC], acc);
+            __syncthreads();
+            if (warp == 0 && c < c_end) {
+                float total[VEC] = {};
+                for (int w = 0; w < kFewWarps; ++w) add_floats<VEC>(total, &part[w][lane * VEC]);
+                write_row<T, VEC>(dw + (static_cast<long long>(row) * shares + blockIdx.x) * f.hidden + c, total, f.scale, f.accumulate);
+            }
+            __syncthreads();
         }
     }
 }
@@ -671,7 +852,7 @@ struct Layout {
 };
 
 bool valid_sizes(std::size_t tokens, std::size_t vocab, std::size_t hidden) {
-    return tokens != 0 && vocab != 0 && hidden != 0 && tokens <= 0x7fffffffull && vocab <= 0x7ffffffeull && hidden <= 0x7fffffffull &&
+    return tokens != 0 && vocab != 0 && hidden != 0 && tokens <= 0x7fffffffull && vocab <= 0x7ffffffeull && hidden <= (1ull << 30) &&
            tokens <= (1ull << 46) / hidden && vocab <= (1ull << 46) / hidden;
 }
 
@@ -698,6 +879,27 @@ int launch_sum(void* dw, const void* dout, GradArgs g, const DropoutArgs& args, 
     CGPT_CUDA_TRY(launch_after_previous(scaled_embedding_join_kernel<T, JV>, dim3(column_tiles * (runs < lanes ? runs : lanes)), kJoinThreads, 0, s,
                                         static_cast<T*>(dw), g));
     count_launch();
+    return CGPT_OK;
+}
+
+bool takes_few(std::size_t tokens, std::size_t vocab, std::size_t hidden, std::size_t elem, bool vectors) {
+    return tokens <= (vectors ? kFewTokens / 2 : kFewTokens) && hidden <= (1u << 20) &&      // a grid has 65535 tiles at most
+           vocab <= (vectors ? (4u << 20) : (16u << 20)) / (hidden * elem);
+}
+
+// Row shares and column tiles of the few-tokens launch: about two CTAs per SM.
+template <typename T, int VEC>
+int launch_few(void* dw, const void* dout, FewArgs f, const DropoutArgs& args, cudaStream_t s) {
+    const int chunk = 32 * VEC;                                          // columns of a warp
+    const int most = f.hidden > (VEC > 1 ? 1 : 4) * chunk ? (VEC > 1 ? 1 : 4) * chunk : f.hidden;
+    const unsigned tiles = static_cast<unsigned>((f.hidden + most - 1) / most);
+    f.tile = most;
+    const unsigned want = tiles < 2 * kNumSMs ? 2 * kNumSMs / tiles : 1, least = (f.vocab + kFewRows - 1) / kFewRows;
+    unsigned shares = want > least ? want : least;
+    if (shares > f.vocab) shares = f.vocab;
+    scaled_embedding_few_kernel<T, VEC><<<dim3(shares, tiles), kFewThreads, 0, s>>>(static_cast<T*>(dw), static_cast<const T*>(dout), f, args);
+    count_launch();
+    CGPT_LAUNCH_CHECK();
     return CGPT_OK;
 }
 
@@ -813,6 +1015,14 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
     auto* base = static_cast<unsigned char*>(workspace);
     auto words = [&](std::size_t offset) { return reinterpret_cast<std::uint32_t*>(base + offset); };
 
+    const bool vectors = hidden % (16 / dtype_size(dtype)) == 0 && aligned16(grad_weight) && aligned16(grad_output);
+    if (takes_few(tokens, vocab, hidden, dtype_size(dtype), vectors)) {
+        const FewArgs f{ids, static_cast<int>(tokens), static_cast<int>(hidden), 0, accumulate, static_cast<std::uint32_t>(vocab), padding_id, scale * args.scale};
+        CGPT_DISPATCH_DTYPE(dtype, T, {
+            if (vectors) return (launch_few<T, 16 / sizeof(T)>(grad_weight, grad_output, f, args, s));
+            return (launch_few<T, 1>(grad_weight, grad_output, f, args, s));
+        });
+    }
     const int bits = bit_length(vocab);   // keys are in [0, vocab]
     const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     const int digit_bits = (bits + passes - 1) / passes;
@@ -870,8 +1080,7 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
     const GradArgs g{c.keys, c.vals, reinterpret_cast<float*>(base + at.partial), c.crossing, static_cast<long long>(tokens),
                      static_cast<long long>(hidden), c.vocab, 0, accumulate, 0, 0, 0, scale * args.scale};
     CGPT_DISPATCH_DTYPE(dtype, T, {
-        constexpr int V = 16 / sizeof(T);
-        if (hidden % V == 0 && aligned16(grad_weight) && aligned16(grad_output)) return (launch_sum<T, V>(grad_weight, grad_output, g, args, s));
+        if (vectors) return (launch_sum<T, 16 / sizeof(T)>(grad_weight, grad_output, g, args, s));
         return (launch_sum<T, 1>(grad_weight, grad_output, g, args, s));
     });
     return CGPT_OK;

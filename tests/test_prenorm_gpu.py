@@ -367,7 +367,9 @@ def backward_case(kind, tokens, vocab, r):
 @pytest.mark.parametrize("tokens,vocab,hidden,dt", [(1, 1, 1, "f32"), (2, 3, 8, "bf16"), (31, 7, 64, "f16"), (32, 1, 40, "f32"), (33, 2, 250, "f32"),
                                                    (64, 600, 16, "bf16"), (777, 1000, 72, "f32"), (2048, 100, 8, "f32"), (2049, 511, 24, "f16"),
                                                    (5000, 40000, 4, "f32"), (10007, 300000, 8, "bf16"), (3000, 77, 1001, "bf16"), (1000, 5, 5000, "bf16"),
-                                                   (9001, 700, 1024, "f16"), (30011, 90, 64, "bf16"), (5003, 2000, 512, "f32")])
+                                                   (1024, 1500, 1032, "bf16"), (1023, 3, 2100, "f32"), (900, 70000, 33, "f16"),
+                                                   (1025, 40, 96, "bf16"), (512, 1500, 1032, "bf16"), (511, 3, 2100, "f32"),
+                                                   (513, 300, 1000, "f16"), (9001, 700, 1024, "f16"), (30011, 90, 64, "bf16"), (5003, 2000, 512, "f32")])
 def test_scaled_embedding_backward(ops, state, kind, tokens, vocab, hidden, dt):
     r = rng(tokens + vocab)
     ids = backward_case(kind, tokens, vocab, r).astype(np.uint32)
