@@ -15,6 +15,7 @@
 // words of the bitmap cost the sort more than it saves).
 //
 // Memory-bound without dropout: backward reads dout once and writes the table once; the sort moves 16 bytes per token and pass.
+// 32768 tokens, 32000 x 1024 bf16: 48 us, with dropout 58: sort and clearing 20, the rest the sums; the decisions make the difference.
 #include <algorithm>
 #include <atomic>
 
@@ -42,7 +43,8 @@ constexpr int kMaxCluster = 16;
 constexpr int kMostKeys = 4;         // keys per thread of the cluster sort
 
 // kLookups consecutive tokens per group of 2^shift threads and trip: their ids, then their rows, are loaded together. What
-// bounds this kernel is the decisions (about 8 of some 12 instructions an element), which are made while rows are on their way.
+// bounds this kernel with dropout is the decisions (15 instructions an element, the integer pipe busy for 61 % of the time), made
+// while rows are on their way: 32768 tokens of 32000 x 1024 bf16 take 27.0 us, 3.2 TB/s of what has to move; 18.4 without dropout.
 constexpr int kLookups = 4;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
@@ -615,15 +617,17 @@ scaled_embedding_join_kernel(T* dw, const GradArgs g) {
 // One launch for few tokens and a small table: sort, sums and joins would be three, of a few microseconds of latency each. A
 // CTA owns every gridDim.x-th row of the table (frequent ids are often neighbours) and a tile of columns. It picks the tokens of
 // its rows out of all ids, in token order, zeroes its rows that have none, and adds up the others, a warp per row; rows with
-// more than kFewOfRow tokens are shared out to all warps afterwards, each taking a part of the list. The order of every sum
+// more than kFewOfRow tokens are shared out to all warps afterwards, each taking a part of the list (16 against 32: 11.7 | 13.4
+// us for 777 tokens of 1000 x 250 f32, 14.8 | 17.0 for 512 of 1024 x 1024 bf16; 8 gives 12.4 and 14.8). The order of every sum
 // follows from the ids alone.
 // The rule (takes_few) by what was measured on both sides, us for one launch against the sort's three, dropout 0.1:
 // vectors, 4 MB table: 1 token f32 1024 wide 8 | 12; 128 tokens f32 256 wide 10 | 14; 512 tokens bf16 1024 wide 17 | 19, f32
 // 768 wide 16 | 21; 1024 tokens 22 | 18; 512 tokens and 8 MB 20 | 19; 32 MB 34 | 21 (rows cleared one by one).
 // Single elements, 513 wide: 1024 tokens f32 4 MB 23 | 33, bf16 16 MB 27 | 33; 1 token, 16 MB 12 | 16. Vectors do best with
 // a warp's width of columns per CTA (four: 33 instead of 27 for 1024 wide), single elements with four.
-constexpr int kFewTokens = 1024, kFewOfRow = 32, kFewThreads = 512, kFewWarps = kFewThreads / 32;
+constexpr int kFewTokens = 1024, kFewOfRow = 16, kFewThreads = 512, kFewWarps = kFewThreads / 32;
 constexpr unsigned kFewRows = 16384;     // rows of a CTA at most (a bit each)
+static_assert(kFewOfRow <= 32, "a warp lists 32 tokens at a time");
 
 struct FewArgs {
     const std::uint32_t* ids;
@@ -682,7 +686,7 @@ scaled_embedding_few_kernel(T* dw, const T* __restrict__ dout, const FewArgs f, 
     __shared__ std::uint32_t token[kFewTokens], row_of[kFewTokens];      // the tokens of this CTA's rows, in token order
     __shared__ std::uint32_t present[kFewRows / 32];
     __shared__ std::uint32_t heads[kFewTokens];                         // list positions at which a row is met first
-    __shared__ std::uint32_t few[kFewWarps][kFewOfRow];                  // per warp: the tokens of the row it adds up
+    __shared__ std::uint32_t few[kFewWarps][32];                         // per warp: the tokens it adds up
     __shared__ int in_warp[kFewWarps], listed, rows_listed;
     __shared__ __align__(16) float part[kFewWarps][32 * VEC];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -814,8 +818,7 @@ struct SumPlan {
         shift = group_shift(hidden, vec);
         const std::size_t group = std::size_t{1} << shift;
         // As many groups as threads allow (and kMostGroups, whose runs are joined one after the other), fewer when there are few
-        // tokens: then every SM gets some. Chunks
-        // as long as lets all CTAs run at once (two per SM), up to kMostChunk.
+        // tokens: then every SM gets some. Chunks as long as lets all CTAs run at once (two per SM), up to kMostChunk.
         const std::size_t slots = 2 * kNumSMs;
         std::size_t n = at_most(kSumThreads / group, kMostGroups);
         n = at_most(n, (tokens + slots * kInFlight - 1) / (slots * kInFlight));
@@ -973,10 +976,10 @@ extern "C" int cgpt_scaled_embedding_forward(void* out, const uint32_t* ids, con
     if (!out || !ids || !weight) return CGPT_ERR_NULL;
     if (!valid_float_dtype(dtype)) return CGPT_ERR_DTYPE;
     if (!valid_sizes(tokens, vocab, hidden)) return CGPT_ERR_SHAPE;
-    if (!std::isfinite(scale)) return CGPT_ERR_OPTION;
     if (!element_aligned(dtype, {out, weight}) || !element_aligned(CGPT_DTYPE_F32, {ids})) return CGPT_ERR_ALIGN;
     DropoutArgs args;
     CGPT_TRY(dropout_args(&args, probability, state, site, tokens * hidden));
+    if (!std::isfinite(scale * args.scale)) return CGPT_ERR_OPTION;      // what kept elements are multiplied by
     auto s = static_cast<cudaStream_t>(stream);
     CGPT_DISPATCH_DTYPE(dtype, T, {
         constexpr int V = 16 / sizeof(T);
@@ -1007,10 +1010,11 @@ extern "C" int cgpt_scaled_embedding_backward(void* grad_weight, const void* gra
     if (!valid_sizes(tokens, vocab, hidden)) return CGPT_ERR_SHAPE;
     const Layout at(tokens, hidden);
     if (workspace_size < at.bytes) return CGPT_ERR_SHAPE;
-    if (!std::isfinite(scale) || grad_weight == grad_output) return CGPT_ERR_OPTION;
+    if (grad_weight == grad_output) return CGPT_ERR_OPTION;
     if (!element_aligned(dtype, {grad_weight, grad_output}) || !element_aligned(CGPT_DTYPE_F32, {ids}) || !aligned16(workspace)) return CGPT_ERR_ALIGN;
     DropoutArgs args;
     CGPT_TRY(dropout_args(&args, probability, state, site, tokens * hidden));
+    if (!std::isfinite(scale * args.scale)) return CGPT_ERR_OPTION;
     auto s = static_cast<cudaStream_t>(stream);
     auto* base = static_cast<unsigned char*>(workspace);
     auto words = [&](std::size_t offset) { return reinterpret_cast<std::uint32_t*>(base + offset); };

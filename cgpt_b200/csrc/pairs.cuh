@@ -82,11 +82,4 @@ __device__ __forceinline__ uint4 to_raw(const Pair (&p)[8 / sizeof(T)]) {
     }
 }
 
-// The pairs of a vector of VEC elements in its packed type, and back.
-template <typename T, int VEC>
-__device__ __forceinline__ void unpack_pairs(Pair (&p)[VEC / 2], const Pack<T, VEC>& pk) {
-    static_assert(sizeof(pk) == 16, "16-byte vectors");
-    to_pairs<T>(p, *reinterpret_cast<const uint4*>(&pk));
-}
-
 }  // namespace cgpt
