@@ -51,8 +51,8 @@ const char* cgpt_b200_version(void);
  * region. */
 uint64_t cgpt_b200_launch_count(void);
 
-/* Reads (and with clear != 0 resets) the device status word of the tensor-core kernels. Every wait in
- * those kernels (on an mbarrier fed by TMA or by tcgen05.commit) is bounded; a kernel whose wait ran out
+/* Reads (and with clear != 0 resets) the device status word of the tensor-core kernels and of the layer norm kernels. Every
+ * wait in those kernels (on an mbarrier fed by TMA, a bulk copy or tcgen05.commit) is bounded; a kernel whose wait ran out
  * sets the word to non-zero and returns. Synchronises the device. */
 int cgpt_b200_device_status(unsigned int* status_out, int clear);
 /* The transformer block's attention branch and MLP branch are independent until the block's last operation (parallel
@@ -293,7 +293,8 @@ int cgpt_add(void* out, const void* a, const void* b, const void* c, size_t coun
  * add, and an embedding with scale and dropout. Their kernels take global scratch from the caller (`workspace`,
  * `workspace_size` bytes, 16-byte aligned; each *_workspace_bytes gives the size, 0 for invalid sizes), so calls on different
  * streams and captured graphs share nothing inside the library. The workspace needs no initial value and holds nothing
- * between calls. Tensors must not overlap unless a parameter says so.
+ * between calls; it serves one call at a time (calls that share one are ordered on a stream). Tensors must not overlap unless a
+ * parameter says so.
  *
  * Dropout. Element e (row-major index) of a call's tensor is decided by 16 bits of Philox4x32-10 with key = seed and counter =
  * (e / 8, site, step low word, step high word): half e % 8 of the block's four words, low halves first. It is kept where those
@@ -340,7 +341,7 @@ int cgpt_dropout_add_layernorm_backward(void* dx, void* dresidual, void* dw, voi
  * Backward: grad_weight[v, :] (+)= scale * sum over tokens t with ids[t] = v of drop(grad_output[t, :]), summed in fp32 in an
  * order that follows from the ids alone and rounded once; tokens whose id is padding_id (UINT32_MAX: none) or outside the table
  * are skipped. accumulate == 0 writes every row of the table (zeros where no token points), else rows without tokens stay as
- * they are. tokens < 2^31. ids: uint32. */
+ * they are. tokens < 2^31, hidden <= 2^30; scale times what kept elements are multiplied by has to be finite. ids: uint32. */
 int cgpt_scaled_embedding_forward(void* out, const uint32_t* ids, const void* weight, size_t tokens, size_t vocab, size_t hidden,
                                   float scale, float probability, const uint64_t* state, uint32_t site, int dtype,
                                   cgpt_stream_t stream);

@@ -150,6 +150,11 @@ def test_refuses_aliases_and_small_workspaces():
     assert lib.cgpt_dropout_advance(None, 1, None) == NULL and lib.cgpt_dropout_advance(A + 4, 1, None) == ALIGN
 
 
+def test_refuses_a_scale_that_overflows_with_dropout():
+    # kept elements are multiplied by scale * 65536 / (65536 - t): infinite here, and 0 * inf in dropped places
+    assert embed_forward(scale=3e38, p=0.5) == OPTION and embed_backward(scale=-3e38, p=0.5) == OPTION
+
+
 def test_python_layer_refuses_host_tensors_and_options():
     x, w, ids = torch.zeros(4, 8), torch.zeros(8), torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError):
