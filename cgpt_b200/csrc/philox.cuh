@@ -30,8 +30,8 @@ struct DropoutArgs {
 
 // The generator of one call. Of a block's counter only the first word differs within a call, so half of the first two rounds is
 // the same for all blocks and worked out once: of the second word's product in round 1 and the first word's in round 2 only what
-// the later rounds XOR in is kept, with the round keys (fused backward 74.7 -> 72.3 us, lookup 28.0 -> 27.0). HOIST: the other round keys are kept in registers too, which saves their
-// additions where registers are free.
+// the later rounds XOR in is kept, with the round keys (fused backward 74.7 -> 72.3 us, lookup 28.0 -> 27.0). HOIST: the other
+// round keys are kept in registers too, which saves their additions where registers are free.
 template <bool HOIST>
 struct PhiloxOf {
     static constexpr std::uint32_t kMul0 = 0xD2511F53u, kMul1 = 0xCD9E8D57u, kKey0 = 0x9E3779B9u, kKey1 = 0xBB67AE85u;
