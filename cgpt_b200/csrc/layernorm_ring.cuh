@@ -14,7 +14,7 @@
 // columns: dx, and the running dw and db of its columns in registers). Lanes that keep both a row's values and dw and db of
 // their columns need 168 registers, and 12 warps an SM hide less: measured 62 against 57 us at 16384 x 2048 bf16.
 //
-// Measured (bf16, device times): forward 32768 x 1024 25.9 us (5.2 TB/s, 80 % of a plain copy's rate; a copy of the same bytes
+// Measured (16-bit, device times): forward 32768 x 1024 25.9 us (5.2 TB/s, 80 % of a plain copy's rate; a copy of the same bytes
 // takes 28.7), with dropout and residual 50 (5.4 TB/s); backward 16384 x 2048 with a residual 54.8 (4.9 TB/s), 32768 x 1024 44.3 (4.5 TB/s),
 // 4096 x 8192 with a residual 65.8 (4.1 TB/s), the fused one at 32768 x 1024 72.3 (4.6 TB/s: bound by instructions, the
 // decisions among them).
