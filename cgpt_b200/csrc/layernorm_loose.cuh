@@ -205,6 +205,8 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
                         if (whole || (c >= begin && c < end)) element(c, keep);
                     }
                 }
+                // columns were dealt out from a generator block's start, below they are from `begin`: lanes read what others wrote
+                __syncwarp();
             } else {
                 each_column(begin, end, lane, [&](int c) { s[0] += to_f32<T>(row[c]); });
             }

@@ -312,6 +312,45 @@ def test_fused_equals_its_parts(ops, state, dt, rows, hidden):
             assert torch.equal(buffer, dr.t)
 
 
+def fused_against_its_parts_and_64_bits(ops, state, rows, hidden, dt):
+    """Both directions of the fused operator: the bits of the two operators it joins, and the 64-bit forms."""
+    x, w, b, dy, res = norm_inputs(rows, hidden, dt)
+    dsum, o = torch.flip(res, (0,)).contiguous(), ops.DropoutOptions(0.2, 6)
+    y, total = Guarded(x.shape, dt), Guarded(x.shape, dt)
+    ops.dropout_add_layernorm_forward(y.t, total.t, x, res, w, b, 1e-5, state, options=o)
+    want_sum, want_y = torch.empty_like(x), torch.empty_like(x)
+    ops.dropout_forward(want_sum, x, state, options=o, residual=res)
+    ops.layernorm_forward(want_y, want_sum, w, b, 1e-5)
+    Y, S, W, B, DY = y.check(), total.check(), host(w), host(b), host(dy)
+    assert torch.equal(total.t, want_sum) and torch.equal(y.t, want_y)
+    dropped = P.drop(host(x), 0.2, SEED, STEP, 6)
+    v = dropped + host(res)
+    close(S, v, P.rounding(v, TORCH[dt]) + 4 * P.U * (np.abs(dropped) + np.abs(v)), "sum")
+    v = P.layernorm(S, W, B, 1e-5)
+    close(Y, v, P.rounding(v, TORCH[dt]) + 2 * P.layernorm_error(S, W, B, 1e-5), "y")
+    dx, dr, dw, db = (Guarded(s, dt) for s in (x.shape, x.shape, w.shape, w.shape))
+    ops.dropout_add_layernorm_backward(dx.t, dr.t, dw.t, db.t, dy, dsum, total.t, w, 1e-5, state, options=o)
+    want = [torch.empty_like(t) for t in (x, w, w)]
+    ops.layernorm_backward(*want, dy, total.t, w, 1e-5, residual=dsum)
+    got = [t.check() for t in (dx, dr, dw, db)]
+    assert all(torch.equal(a.t, v) for a, v in zip((dr, dw, db), want))
+    (d, *sums), (err, *sum_err) = P.layernorm_backward(DY, S, W, 1e-5), P.layernorm_backward_error(DY, S, W, 1e-5)
+    d, size = d + host(dsum), np.abs(host(dsum))
+    err = 2 * err + 2 * P.U * (size + np.abs(d))
+    close(got[1], d, P.rounding(d, TORCH[dt]) + err, "dresidual")
+    v = P.drop(d, 0.2, SEED, STEP, 6)
+    close(got[0], v, P.rounding(v, TORCH[dt]) + 1.3 * err + 3 * P.U * np.abs(v), "dx")
+    for a, v, e, what in zip(got[2:], sums, sum_err, ("dw", "db")):
+        close(a, v, P.rounding(v, TORCH[dt]) + 2 * e, what)
+
+
+@pytest.mark.parametrize("rows,hidden,dt", [(12000, 1001, "bf16"), (20000, 511, "f16"), (5000, 1001, "f32"), (2000, 4099, "bf16")])
+def test_fused_odd_rows_through_refilled_stages(ops, state, rows, hidden, dt):
+    """Enough rows that every stage of a ring is filled again after its sums were written over what it held; one warp per row and
+    several, more than one row a stage."""
+    fused_against_its_parts_and_64_bits(ops, state, rows, hidden, dt)
+
+
 @pytest.mark.parametrize("hidden", [512, 511, 3000, 2999, 20000])
 def test_fused_in_place_sum_and_no_dropout(ops, state, hidden):
     x, w, b, _, res = norm_inputs(1200, hidden, "f16")
