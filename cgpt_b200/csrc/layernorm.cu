@@ -14,10 +14,10 @@
 // Memory-bound: 2 * H * sizeof(T) bytes per row forward, 3 backward (+1 with a residual), 4 and 5 for the fused pair.
 #include <type_traits>
 
+#include "bulk_ring.cuh"
 #include "dependent_launch.cuh"
 #include "philox.cuh"
 #include "launch_counter.h"
-#include "sm100.cuh"
 
 namespace cgpt {
 

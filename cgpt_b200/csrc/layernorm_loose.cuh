@@ -46,20 +46,8 @@ __host__ __device__ __forceinline__ Span span_of(const T* tensor, long long row0
     return s;
 }
 
-// Ring of stages of up to three tensors, as ring_kernels::Ring.
-struct Ring {
-    unsigned char* data;
-    std::uint64_t* full;
-    unsigned int* status;
-    unsigned stage_bytes, tensor_bytes;
-    int stages, stage;
-    std::uint32_t parity;
-    bool failed;
-
-    __device__ __forceinline__ void init() const {
-        for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[s], 1);
-        sm100::mbar_init_fence();
-    }
+// Ring of stages of consecutive rows of up to three tensors, each where its span has it.
+struct Ring : BulkRing {
     template <typename T>
     __device__ __forceinline__ void fill(int s, const T* a, const T* b, const T* c, long long row0, int step_rows, long long rows, int hidden) const {
         if (row0 >= rows) return;
@@ -71,23 +59,6 @@ struct Ring {
         if (sa.bytes != 0) sm100::bulk_load_1d(to + sa.at, sa.from, sa.bytes, &full[s]);
         if (sb.bytes != 0) sm100::bulk_load_1d(to + tensor_bytes + sb.at, sb.from, sb.bytes, &full[s]);
         if (sc.bytes != 0) sm100::bulk_load_1d(to + 2 * tensor_bytes + sc.at, sc.from, sc.bytes, &full[s]);
-    }
-    __device__ __forceinline__ unsigned char* wait() {
-        if (!failed && !sm100::mbar_wait(&full[stage], parity)) {
-            failed = true;
-            atomicExch(status, 5u);
-        }
-        return data + stage * stage_bytes;
-    }
-    __device__ __forceinline__ void next() {
-        if (++stage == stages) { stage = 0; parity ^= 1u; }
-    }
-    // Before the CTA leaves: copies that a failed wait gave up on get time to land while the memory is still its own.
-    __device__ __forceinline__ void leave() const {
-        if (failed) {
-            const unsigned long long t0 = sm100::globaltimer_ns();
-            while (sm100::globaltimer_ns() - t0 < 200000ull) { }
-        }
     }
 };
 

@@ -32,21 +32,10 @@ constexpr std::size_t kStatsBytes = 2 * kMaxTileRows * 32;   // static shared me
 // Rows a warp group takes at a time: a lane with few vectors per row holds several rows.
 __host__ __device__ constexpr int rows_at_once(int cpt) { return cpt >= 4 ? 1 : 4 / cpt; }
 
-// A ring of stages. A wait that runs out sets the library's status word; the CTA then goes on with what is there (every barrier
-// is still met, nothing is written out of bounds) and waits no more.
-struct Ring {
-    unsigned char* data;
-    std::uint64_t* full;
-    unsigned int* status;
-    unsigned stage_bytes, tensor_bytes, row_bytes;
-    int stages, stage;
-    std::uint32_t parity;
-    bool failed;
+// Ring of stages of consecutive rows of up to three tensors.
+struct Ring : BulkRing {
+    unsigned row_bytes;
 
-    __device__ __forceinline__ void init() const {   // by one thread, before the CTA's first barrier
-        for (int s = 0; s < stages; ++s) sm100::mbar_init(&full[s], 1);
-        sm100::mbar_init_fence();
-    }
     // Rows row0 .. row0 + step_rows of a, b and c (b and c may be null) into stage s, as far as there are such rows.
     template <typename T>
     __device__ __forceinline__ void fill(int s, const T* a, const T* b, const T* c, long long row0, int step_rows, long long rows, int hidden) const {
@@ -57,23 +46,6 @@ struct Ring {
         sm100::bulk_load_1d(to, a + row0 * hidden, n, &full[s]);
         if (b != nullptr) sm100::bulk_load_1d(to + tensor_bytes, b + row0 * hidden, n, &full[s]);
         if (c != nullptr) sm100::bulk_load_1d(to + 2 * tensor_bytes, c + row0 * hidden, n, &full[s]);
-    }
-    __device__ __forceinline__ const unsigned char* wait() {
-        if (!failed && !sm100::mbar_wait(&full[stage], parity)) {
-            failed = true;
-            atomicExch(status, 5u);
-        }
-        return data + stage * stage_bytes;
-    }
-    __device__ __forceinline__ void next() {
-        if (++stage == stages) { stage = 0; parity ^= 1u; }
-    }
-    // Before the CTA leaves: copies that a failed wait gave up on get time to land while the memory is still its own.
-    __device__ __forceinline__ void leave() const {
-        if (failed) {
-            const unsigned long long t0 = sm100::globaltimer_ns();
-            while (sm100::globaltimer_ns() - t0 < 200000ull) { }
-        }
     }
 };
 
