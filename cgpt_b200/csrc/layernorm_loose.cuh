@@ -127,6 +127,7 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
     const long long step = static_cast<long long>(gridDim.x) * la.groups * la.step_rows;
     const long long first = (static_cast<long long>(blockIdx.x) * la.groups + group) * la.step_rows;
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
+    bool leader = tid == 0;
     Ring ring{};
     ring.tensor_bytes = la.tensor_bytes;
     ring.stage_bytes = FUSED ? 2 * la.tensor_bytes : la.tensor_bytes;
@@ -135,7 +136,7 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
     ring.data = shared + la.data_offset + static_cast<std::size_t>(group) * la.stages * ring.stage_bytes;
     ring.status = la.status;
     const T *second = FUSED ? residual : nullptr, *none = nullptr;
-    if (tid == 0) {
+    if (leader) {
         ring.init();
         for (int s = 0; s < la.stages; ++s) ring.fill(s, x, second, none, first + s * step, la.step_rows, rows, hidden);
     }
@@ -145,7 +146,7 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
     __syncthreads();
 
     for (long long row0 = first; row0 < rows; row0 += step) {
-        unsigned char* stage = ring.wait();
+        unsigned char* stage = ring.wait(&leader);
         const unsigned n = static_cast<unsigned>(rows - row0 < la.step_rows ? rows - row0 : la.step_rows);
         T *xs, *rs = nullptr;
         bool loaded = complete(xs, stage, x, row0, n, rows, hidden, tid, lanes);
@@ -197,10 +198,9 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
         }
         if constexpr (FUSED) stores_before_copies();
         meet(la.warps_per_row, group + 1);
-        if (tid == 0) ring.fill(ring.stage, x, second, none, row0 + ring.stages * step, la.step_rows, rows, hidden);
+        if (leader) ring.fill(ring.stage, x, second, none, row0 + ring.stages * step, la.step_rows, rows, hidden);
         ring.next();
     }
-    ring.leave();
 }
 
 // Tiles of rows in two phases, as ring_kernels: a warp group per row for the sums, then a thread per column. K columns per thread,
@@ -270,7 +270,7 @@ layernorm_backward_loose_kernel(T* dx, T* din, float* __restrict__ partial, cons
         }
         __syncthreads();
         // Every thread is past the columns of the tile before: its stage is free.
-        if (threadIdx.x == 0 && row0 != first)
+        if (threadIdx.x == 0 && !ring.failed && row0 != first)
             ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, residual, row0 + (ring.stages - 1) * step, la.step_rows, rows, hidden);
         // ---- columns: RJ rows (of the row group) at a time; with dropout the lanes of a warp share the decisions of four elements
         constexpr int RJ = K >= 4 ? 1 : 4 / K;
@@ -315,14 +315,14 @@ layernorm_backward_loose_kernel(T* dx, T* din, float* __restrict__ partial, cons
         }
         ring.next();
     }
-    ring.leave();
     // One partial row of dw and of db per CTA: its row groups add up one after the other, in the memory of the ring, whose copies
-    // have all been waited for.
+    // have all been waited for. Where a wait ran out they may not have come, and the rows are worth nothing.
+    if (__syncthreads_or(ring.failed)) return;
     float* out_w = partial + static_cast<long long>(blockIdx.x) * 2 * hidden;
     float* joined = reinterpret_cast<float*>(shared + la.data_offset);
     const int groups = K == 1 ? la.groups : 1;
     for (int q = 0; q < groups; ++q) {
-        __syncthreads();
+        if (q > 0) __syncthreads();
         if (works && row_group == q) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {

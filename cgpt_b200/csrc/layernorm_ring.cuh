@@ -135,7 +135,7 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
     const long long step = static_cast<long long>(gridDim.x) * ra.groups * ra.step_rows;
     const long long first = (static_cast<long long>(blockIdx.x) * ra.groups + group) * ra.step_rows;
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
-    const bool leader = warp_in_row == 0 && lane == 0;
+    bool leader = warp_in_row == 0 && lane == 0;
     Ring ring{};
     ring.row_bytes = static_cast<unsigned>(hidden) * sizeof(T);
     ring.tensor_bytes = ra.step_rows * ring.row_bytes;
@@ -156,7 +156,7 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
     __syncthreads();
 
     for (long long row0 = first; row0 < rows; row0 += step) {
-        const unsigned char* at = ring.wait() + lane_bytes;
+        const unsigned char* at = ring.wait(&leader) + lane_bytes;
         const int left = rows - row0 < ra.step_rows ? static_cast<int>(rows - row0) : ra.step_rows;   // rows of this step
         const long long e0 = (row0 + lane_row) * hidden + vec0 * VEC;                                 // the lane's first element
         Pair v[R][CPT][NP];
@@ -236,7 +236,6 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
             }
         }
     }
-    ring.leave();
 }
 
 // CPT: vectors per lane in the row phase (FULL: exactly the row's). COLS: vectors per thread and row in the column phase.
@@ -384,7 +383,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
         }
         __syncthreads();
         // Every thread is past the columns of the tile before: its stage is free.
-        if (threadIdx.x == 0 && row0 != first)
+        if (threadIdx.x == 0 && !ring.failed && row0 != first)
             ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, none, row0 + (ring.stages - 1) * step, ra.step_rows, rows, hidden);
         // ---- columns
         auto columns = [&](auto all_rows) {
@@ -428,15 +427,15 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
         }
         ring.next();
     }
-    ring.leave();
 
     // One partial row of dw and of db per CTA: its row groups add up one after the other, in the memory of the ring, whose copies
-    // have all been waited for.
+    // have all been waited for. Where a wait ran out they may not have come, and the rows are worth nothing.
+    if (__syncthreads_or(ring.failed)) return;
     float* out_w = partial + static_cast<long long>(blockIdx.x) * 2 * hidden;
     Pair* joined = reinterpret_cast<Pair*>(shared + ra.data_offset);           // [pair][dw, db][vector]: no bank conflicts
     const int groups = COLS == 1 ? ra.groups : 1;
     for (int k = 0; k < groups; ++k) {
-        __syncthreads();
+        if (k > 0) __syncthreads();
         if (works && row_group == k) {
 #pragma unroll
             for (int c = 0; c < COLS; ++c) {

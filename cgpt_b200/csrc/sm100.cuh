@@ -48,13 +48,13 @@ __device__ __forceinline__ bool mbar_try_wait(std::uint64_t* bar, std::uint32_t 
         : "memory");
     return ok != 0;
 }
-// Waits for the phase with the given parity to complete. Returns false after kWaitLimitNs.
-__device__ __forceinline__ bool mbar_wait(std::uint64_t* bar, std::uint32_t parity) {
+// Waits for the phase with the given parity to complete. Returns false after limit_ns.
+__device__ __forceinline__ bool mbar_wait(std::uint64_t* bar, std::uint32_t parity, unsigned long long limit_ns = kWaitLimitNs) {
     if (mbar_try_wait(bar, parity)) return true;
     const unsigned long long start = globaltimer_ns();
     unsigned spins = 0;
     while (!mbar_try_wait(bar, parity)) {
-        if ((++spins & 1023u) == 0 && globaltimer_ns() - start > kWaitLimitNs) return false;
+        if ((++spins & 1023u) == 0 && globaltimer_ns() - start > limit_ns) return false;
     }
     return true;
 }
