@@ -813,19 +813,25 @@ std::size_t at_most(std::size_t n, std::size_t limit) { return n < limit ? n : l
 
 // Layout of the run sums: threads per row (2^shift), groups per CTA, CTAs.
 struct SumPlan {
+    static constexpr std::size_t kSlots = 2 * kNumSMs;       // CTAs that run at once
     int shift, groups, chunk, ctas;
     SumPlan(std::size_t tokens, std::size_t hidden, int vec) {
         shift = group_shift(hidden, vec);
-        const std::size_t group = std::size_t{1} << shift;
         // As many groups as threads allow (and kMostGroups, whose runs are joined one after the other), fewer when there are few
         // tokens: then every SM gets some. Chunks as long as lets all CTAs run at once (two per SM), up to kMostChunk.
-        const std::size_t slots = 2 * kNumSMs;
-        std::size_t n = at_most(kSumThreads / group, kMostGroups);
-        n = at_most(n, (tokens + slots * kInFlight - 1) / (slots * kInFlight));
+        std::size_t n = at_most(most_groups(shift), (tokens + kSlots * kInFlight - 1) / (kSlots * kInFlight));
         groups = static_cast<int>(n);
-        const std::size_t even = (tokens + slots * n - 1) / (slots * n);
+        const std::size_t even = (tokens + kSlots * n - 1) / (kSlots * n);
         chunk = static_cast<int>(even < kMostChunk ? (even + kInFlight - 1) / kInFlight * kInFlight : kMostChunk);
         ctas = static_cast<int>((tokens + n * chunk - 1) / (n * chunk));
+    }
+    static std::size_t most_groups(int shift) { return at_most(kSumThreads >> shift, kMostGroups); }
+    // The most CTAs of a plan for up to `tokens` tokens. (`ctas` itself falls where CTAs get another group.) A CTA has kInFlight
+    // tokens at least. Shorter chunks than kMostChunk are as long as lets all CTAs run at once; a plan that needs the longest has
+    // all groups by then: it takes more than 31 kSlots tokens a group, and kInFlight kSlots tokens make a group.
+    static std::size_t most_ctas(std::size_t tokens, std::size_t hidden, int vec) {
+        const std::size_t span = most_groups(group_shift(hidden, vec)) * kMostChunk;
+        return std::max(at_most((tokens + kInFlight - 1) / kInFlight, kSlots), (tokens + span - 1) / span);
     }
 };
 
@@ -836,10 +842,7 @@ struct Layout {
     Layout(std::size_t tokens, std::size_t hidden) {
         tiles = static_cast<int>((tokens + kSortTile - 1) / kSortTile);
         std::size_t ctas = 0;
-        for (int vec : {1, 4, 8}) {
-            const SumPlan p(tokens, hidden, vec);
-            if (static_cast<std::size_t>(p.ctas) > ctas) ctas = p.ctas;
-        }
+        for (int vec : {1, 4, 8}) ctas = std::max(ctas, SumPlan::most_ctas(tokens, hidden, vec));
         bytes = 0;
         auto take = [&](std::size_t n) {
             const std::size_t at = bytes;

@@ -310,12 +310,16 @@ RingPlan plan_forward_ring(std::size_t rows, std::size_t hidden, std::size_t ele
     return p;
 }
 
+// Threads of a CTA of the backward; kBackwardThreads in all on an SM.
+int backward_ring_threads(std::size_t vectors) { return vectors <= 256 ? 256 : ring_kernels::kBackwardThreads; }
+int backward_loose_threads(std::size_t hidden) { return hidden <= 2048 ? 256 : loose_kernels::kBackwardThreads; }
+
 // Threads cover as many rows at a time as they have vectors for, fewer when there are few rows.
 RingPlan plan_backward_ring(std::size_t rows, std::size_t hidden, std::size_t elem) {
     RingPlan p = plan_row(hidden, elem, 4);
     auto& a = p.args;
     const std::size_t v = a.vectors;
-    p.threads = v <= 256 ? 256 : ring_kernels::kBackwardThreads;
+    p.threads = backward_ring_threads(v);
     p.cols = v <= 512 ? 1 : v <= 1024 ? 2 : 4;
     const std::size_t ctas = ring_kernels::kBackwardThreads / p.threads, rows_each = ring_kernels::kTileVectors / p.cols;
     std::size_t groups = p.cols == 1 ? p.threads / v : 1;
@@ -365,7 +369,7 @@ LoosePlan plan_forward_loose(std::size_t rows, std::size_t hidden, std::size_t e
 LoosePlan plan_backward_loose(std::size_t rows, std::size_t hidden, std::size_t elem) {
     LoosePlan p{};
     auto& a = p.args;
-    p.threads = hidden <= 2048 ? 256 : loose_kernels::kBackwardThreads;
+    p.threads = backward_loose_threads(hidden);
     p.columns = 1;
     while (static_cast<std::size_t>(p.columns) * p.threads < hidden) p.columns *= 2;
     const std::size_t ctas = loose_kernels::kBackwardThreads / p.threads;
@@ -415,14 +419,17 @@ int allow_smem(Kernel kernel, PerDeviceOnce* once, std::size_t fixed = 0) {
     return CGPT_OK;
 }
 
-// Enough for the call's layout whatever its type and alignment turn out to be.
+// Enough for the call's layout whatever its type and alignment turn out to be, and for every call with fewer rows: a CTA has a row
+// at least, and no more CTAs are launched than the SMs hold. (A plan's own grid falls where a CTA starts to take more rows.)
 std::size_t workspace_bytes(std::size_t rows, std::size_t hidden) {
     std::size_t parts = 0, stats = 0;
     for (std::size_t elem : {2, 4})
         for (bool vector : {false, true}) {
             const Form form = form_of(hidden, elem, vector);
-            const std::size_t n = form == Form::kRing ? plan_backward_ring(rows, hidden, elem).grid
-                                  : form == Form::kLoose ? plan_backward_loose(rows, hidden, elem).grid : any_splits(rows);
+            const std::size_t ring_ctas = ring_kernels::kBackwardThreads / backward_ring_threads(hidden * elem / 16);
+            const std::size_t loose_ctas = loose_kernels::kBackwardThreads / backward_loose_threads(hidden);
+            const std::size_t n = form == Form::kRing ? at_most(rows, kNumSMs * ring_ctas)
+                                  : form == Form::kLoose ? at_most(rows, kNumSMs * loose_ctas) : any_splits(rows);
             if (n > parts) parts = n;
             if (form == Form::kAny) stats = rows * sizeof(float2);
         }

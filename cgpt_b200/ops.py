@@ -573,7 +573,7 @@ def layernorm_backward(grad_input, grad_weight, grad_bias, grad_output, input, w
 
 
 def layernorm_backward_workspace_bytes(rows: int, hidden: int) -> int:
-    """Workspace of layernorm_backward and dropout_add_layernorm_backward."""
+    """Workspace of layernorm_backward and dropout_add_layernorm_backward; enough for fewer rows of this width too."""
     return lib.cgpt_layernorm_backward_workspace_bytes(rows, hidden)
 
 
@@ -644,6 +644,7 @@ def scaled_embedding_backward(grad_weight, grad_output, device_token_ids, token_
 
 
 def scaled_embedding_backward_workspace_bytes(token_count: int, hidden: int) -> int:
+    """Workspace of scaled_embedding_backward; enough for fewer tokens of this width too."""
     return lib.cgpt_scaled_embedding_backward_workspace_bytes(token_count, hidden)
 
 

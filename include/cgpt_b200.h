@@ -292,8 +292,8 @@ int cgpt_add(void* out, const void* a, const void* b, const void* c, size_t coun
  * Operators of the pre-norm block that the reference does not have: dropout, layer norm, the two fused with the residual
  * add, and an embedding with scale and dropout. Their kernels take global scratch from the caller (`workspace`,
  * `workspace_size` bytes, 16-byte aligned; each *_workspace_bytes gives the size, 0 for invalid sizes), so calls on different
- * streams and captured graphs share nothing inside the library. The workspace needs no initial value and holds nothing
- * between calls; it serves one call at a time (calls that share one are ordered on a stream). Tensors must not overlap unless a
+ * streams and captured graphs share nothing inside the library. The size never falls with more rows (tokens) of one width: a
+ * buffer for the largest batch serves every smaller one. The workspace needs no initial value and holds nothing between calls; it serves one call at a time (calls that share one are ordered on a stream). Tensors must not overlap unless a
  * parameter says so.
  *
  * Dropout. Element e (row-major index) of a call's tensor is decided by 16 bits of Philox4x32-10 with key = seed and counter =

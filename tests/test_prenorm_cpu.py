@@ -51,6 +51,14 @@ def test_workspace_sizes():
     assert size(1, 1) >= 16
 
 
+@pytest.mark.parametrize("size", [lib.cgpt_layernorm_backward_workspace_bytes, lib.cgpt_scaled_embedding_backward_workspace_bytes])
+@pytest.mark.parametrize("hidden", [1, 64, 250, 256, 511, 1000, 1024, 2048, 2056, 4099, 8192, 12008, 16384])
+def test_a_workspace_for_many_rows_serves_fewer(size, hidden):
+    """Rows a CTA takes, and CTAs, change with the row count; what is asked for may not fall at any of these changes."""
+    sizes = [size(n, hidden) for n in (*range(1, 12000), *range(12000, 80000, 37))]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
 def dropout_forward(out=A, x=B, residual=None, count=8, p=0.5, state=C, site=0, dtype=BF16):
     return lib.cgpt_dropout_forward(out, x, residual, count, p, state, site, dtype, None)
 

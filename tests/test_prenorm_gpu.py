@@ -636,3 +636,22 @@ def test_explicit_stream_and_caller_workspace(ops, state):
     ops.layernorm_backward(*got, dy, x, w, 1e-5, stream=stream)
     stream.synchronize()
     assert all(torch.equal(a, v) for a, v in zip(got, want))
+
+
+@pytest.mark.parametrize("hidden", [256, 1001, 1024])
+def test_one_workspace_for_the_largest_batch(ops, state, hidden):
+    """A workspace for the most rows serves all smaller calls: the bits are those of a call with its own."""
+    most = 1300
+    x, w, _, dy, _ = norm_inputs(most, hidden, "bf16")
+    ids, o = ids_dev(rng(2).integers(0, 3000, most).astype(np.uint32)), ops.ScaledEmbeddingOptions(2.0, dropout=ops.DropoutOptions(0.1, 3))
+    for_norm = torch.empty(ops.layernorm_backward_workspace_bytes(most, hidden), device="cuda", dtype=torch.uint8)
+    for_table = torch.empty(ops.scaled_embedding_backward_workspace_bytes(most, hidden), device="cuda", dtype=torch.uint8)
+    for n in (1, 2, 147, 296, 297, 591, 593, 1183, 1184, 1185, most):
+        want, got = ([torch.full_like(t, float("nan")) for t in (x[:n], w, w)] for _ in range(2))
+        ops.layernorm_backward(*want, dy[:n], x[:n], w, 1e-5)
+        ops.layernorm_backward(*got, dy[:n], x[:n], w, 1e-5, workspace=for_norm)
+        assert all(torch.equal(a, v) for a, v in zip(got, want))
+        want, got = (torch.full((3000, hidden), float("nan"), device="cuda", dtype=x.dtype) for _ in range(2))
+        ops.scaled_embedding_backward(want, dy[:n], ids, n, state, options=o)
+        ops.scaled_embedding_backward(got, dy[:n], ids, n, state, options=o, workspace=for_table)
+        assert torch.equal(got, want)
