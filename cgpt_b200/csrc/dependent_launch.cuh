@@ -1,7 +1,9 @@
 // Programmatic dependent launch of the later kernels of one operator: the launch is prepared, and its CTAs placed where there is
 // room, while the kernel before it in the stream still runs. The first kernel calls launch_dependents() as soon as it starts, the
 // later one wait_for_previous() before it touches anything the first one writes or reads: it returns when that kernel has
-// finished and its writes are visible. Kernels of other operators are launched normally, after all of this.
+// finished and its writes are visible. To ordinary loads: a parameter that points to what the first kernel writes must not be
+// `const __restrict__`, which allows loads that count on memory that stays as it is from the launch on. Kernels of other operators
+// are launched normally, after all of this.
 #pragma once
 
 #include <utility>

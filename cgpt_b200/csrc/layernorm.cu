@@ -227,7 +227,7 @@ layernorm_columns_any_kernel(float* __restrict__ partial, const T* __restrict__ 
 // chooses dw or db.
 template <typename T>
 __global__ void __launch_bounds__(1024)
-layernorm_reduce_kernel(T* __restrict__ dw, T* __restrict__ db, const float* __restrict__ partial, int parts, long long hidden) {
+layernorm_reduce_kernel(T* dw, T* db, const float* partial, int parts, long long hidden) {
     __shared__ float tile[32][33];
     const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const long long col = static_cast<long long>(blockIdx.x) * 32 + lane;
