@@ -476,9 +476,10 @@ def _dropout_options(name, options, state, device):
 
 
 # These calls take a few microseconds of host time on a small tensor, most of it here: the checks below read each property once,
-# build no message unless they fail, and take the current stream's pointer directly (0.2 us; through torch.cuda.Stream 3.6 us).
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# build no message unless they fail, and take the current stream's pointer directly where torch gives it (0.2 us; through
+# torch.cuda.Stream 3.6 us). A torch without CUDA has no such function: the module is imported there all the same.
+_current_device = torch.cuda.current_device
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _stream_on(name, device, stream):

@@ -1,6 +1,9 @@
 """Host side of the pre-norm block's operators: the generator's published vectors, formulas against differences, workspace sizes,
 and every refusal of the C ABI and of the Python layer. No kernel is launched: each call below is refused before it would."""
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -186,3 +189,13 @@ def test_python_layer_refuses_host_tensors_and_options():
 def test_state_holds_any_64_bit_words():
     s = ops.make_dropout_state(0xffffffffffffffff, 1 << 63, device="cpu")
     assert [ctypes.c_uint64(v).value for v in s.tolist()] == [0xffffffffffffffff, 1 << 63]
+
+
+def test_the_module_is_imported_without_cuda_functions_in_torch():
+    """What a torch built without CUDA lacks is taken away in a fresh process before the import."""
+    code = ("import torch\nfor name in dir(torch._C):\n    if name.startswith('_cuda_'): delattr(torch._C, name)\n"
+            "import cgpt_b200.ops as ops\n"
+            "try: ops.layernorm_forward(*(torch.zeros(4, 8) for _ in range(2)), torch.zeros(8), None, 1e-5)\n"
+            "except ValueError: print('refused')\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True)
+    assert done.stdout == "refused\n", done.stderr
