@@ -946,8 +946,8 @@ int most_cluster_ctas(int* ctas) {
         cudaLaunchAttribute attribute;
         CGPT_TRY(cluster_config(&config, &attribute, 2, kMaxCluster, nullptr));
         int n = 0;
-        const bool fits = cudaOccupancyMaxActiveClusters(&n, kClusterKernels[2], &config) == cudaSuccess && n > 0;
-        cudaGetLastError();
+        const bool asked = cudaOccupancyMaxActiveClusters(&n, kClusterKernels[2], &config) == cudaSuccess, fits = asked && n > 0;
+        if (!asked) cudaGetLastError();       // its own error only: an earlier one is the caller's to read
         *ctas = fits ? kMaxCluster : 8;
         known[device].store(*ctas, std::memory_order_relaxed);
     }

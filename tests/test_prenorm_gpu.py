@@ -655,3 +655,19 @@ def test_one_workspace_for_the_largest_batch(ops, state, hidden):
         ops.scaled_embedding_backward(want, dy[:n], ids, n, state, options=o)
         ops.scaled_embedding_backward(got, dy[:n], ids, n, state, options=o, workspace=for_table)
         assert torch.equal(got, want)
+
+
+def test_the_callers_last_error_is_left_alone(ops):
+    """A gradient through the sort between a refused runtime call and the caller's look at its error. (Not the first in its process:
+    the runtime itself clears the error where it sets a kernel's attributes, once per device.)"""
+    from cgpt_b200 import _lib
+    runtime, ids, grad = _lib.lib, torch.zeros(2000, dtype=torch.int32, device="cuda"), torch.ones(2000, 64, device="cuda")
+    table, size = torch.empty(50000, 64, device="cuda"), ops.scaled_embedding_backward_workspace_bytes(2000, 64)
+    workspace, stream = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.cuda.current_stream().cuda_stream
+    call = lambda: _lib.lib.cgpt_scaled_embedding_backward(table.data_ptr(), grad.data_ptr(), ids.data_ptr(), workspace.data_ptr(), size, 2000,
+                                                           50000, 64, 1.0, 0xffffffff, 0.0, None, 0, 0, _lib.F32, stream)
+    assert call() == 0
+    refused = runtime.cudaSetDevice(-1)
+    rc, seen = call(), runtime.cudaGetLastError()
+    assert rc == 0 and refused != 0 and seen == refused
+    assert bool((table[0] == 2000).all()) and not bool(table[1:].any())
