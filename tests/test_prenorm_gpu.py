@@ -433,6 +433,47 @@ def test_scaled_embedding_backward(ops, state, kind, tokens, vocab, hidden, dt):
             assert torch.equal(got[0][untouched], before[untouched])
 
 
+@pytest.mark.parametrize("kind", ["uniform", "same", "skewed", "outside", "none"])
+@pytest.mark.parametrize("tokens,vocab,hidden,dt,shift", [(65537, 500, 8, "f32", 0), (70001, 511, 5, "bf16", 0), (70003, 40000, 8, "bf16", 0), (66000, 3000, 24, "f16", 1),
+                                                         (100003, 300000, 4, "f32", 0), (68000, 262144, 3, "f16", 1)])
+def test_scaled_embedding_backward_of_many_tokens(ops, state, kind, tokens, vocab, hidden, dt, shift):
+    """More tokens than one cluster sorts: count, prefix and scatter launches, one, two and three passes of them, the table cleared
+    by itself; ids outside the table, a padding id, accumulation, dropout, tensors off the 16-byte grid."""
+    r = rng(tokens)
+    ids = backward_case(kind, tokens, vocab, r).astype(np.uint32)
+    grad, before = shifted(r.standard_normal((tokens, hidden)), dt, shift), dev(r.standard_normal((vocab, hidden)), dt)
+    for p, padding, accumulate in ((0.0, None, False), (0.3, int(ids[0]) if ids[0] < vocab else 0, False), (0.3, None, True)):
+        o = ops.ScaledEmbeddingOptions(1.75, padding, ops.DropoutOptions(p, 8), accumulate)
+        table, size, count = P.embedding_backward(ids, P.drop(host(grad), p, SEED, STEP, 8), vocab, 1.75, padding)
+        got = []
+        for _ in range(2):
+            out = Guarded((vocab, hidden), dt, shift)
+            if accumulate:
+                out.t.copy_(before)
+            ops.scaled_embedding_backward(out.t, grad, ids_dev(ids), tokens, state, options=o)
+            want = table + (host(before) if accumulate else 0)
+            close(out.check(), want, P.rounding(want, TORCH[dt]) + P.U * ((count[:, None] + 8) * size + 2 * np.abs(want)), "grad_weight")
+            got.append(out.t)
+        assert torch.equal(*got)
+        if accumulate:
+            untouched = torch.from_numpy(count == 0).cuda()
+            assert torch.equal(got[0][untouched], before[untouched])
+
+
+@pytest.mark.parametrize("vocab", [400, 50000, 400000])
+def test_both_sorts_keep_the_tokens_in_order(ops, state, vocab):
+    """The same tokens through the cluster sort, and, with 64 skipped ones behind them, through the launches per digit. Both counts
+    are summed in chunks of equal length, so the bits are the same exactly if the sorted tokens are."""
+    tokens, hidden, more = 65536, 8, 64
+    r = rng(vocab)
+    ids, grad = backward_case("skewed", tokens, vocab, r), r.standard_normal((tokens + more, hidden))
+    o, g = ops.ScaledEmbeddingOptions(1.5, dropout=ops.DropoutOptions(0.2, 4)), dev(grad, "f32")
+    a, b = (torch.empty(vocab, hidden, device="cuda") for _ in range(2))
+    ops.scaled_embedding_backward(a, g[:tokens], ids_dev(ids), tokens, state, options=o)
+    ops.scaled_embedding_backward(b, g, ids_dev(np.concatenate([ids, vocab + np.arange(more)])), tokens + more, state, options=o)
+    assert torch.equal(a, b)
+
+
 def test_scaled_embedding_backward_of_unaligned_tensors(ops):
     r = rng(5)
     ids = r.integers(0, 40, 500).astype(np.uint32)
