@@ -248,8 +248,8 @@ layernorm_reduce_kernel(T* dw, T* db, const float* partial, int parts, long long
 #include "layernorm_ring.cuh"
 #include "layernorm_loose.cuh"
 
-// How a call's rows are laid out. It follows from the sizes and the alignment alone, not from which operator is called, so that
-// the fused operators give the bits of their parts.
+// How a call's rows are laid out. It follows from the sizes and the alignment of all its tensors alone, not from which operator is
+// called, so that the fused operators give the bits of their parts for tensors of like alignment.
 enum class Form { kAny, kLoose, kRing };
 
 constexpr std::size_t kSmemPerSm = 227 * 1024;

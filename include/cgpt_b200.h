@@ -325,8 +325,10 @@ int cgpt_layernorm_backward(void* dx, void* dw, void* db, const void* dy, const 
                             cgpt_stream_t stream);
 
 /* Sub-layer boundary of a pre-norm block in one pass:  sum = residual + drop(x), y = layernorm(sum), both written; the norm is
- * of the rounded sum, so results equal cgpt_dropout_forward followed by cgpt_layernorm_forward. sum may be the same buffer as
- * x or residual. Backward takes the gradient of y and (unless NULL) that of sum from the residual path:
+ * of the rounded sum, so the results are those of cgpt_dropout_forward followed by cgpt_layernorm_forward: sum bit for bit, y too
+ * where all tensors are 16-byte aligned or one of y, sum, w and b is not (rows are added in another order where an unaligned tensor
+ * is among the arguments, and x and residual are not arguments of the second call). sum may be the same buffer as x or residual.
+ * Backward takes the gradient of y and (unless NULL) that of sum from the residual path:
  *      dresidual = dsum + layernorm_backward(dy; sum, w),  dx = drop(dresidual before its rounding),  dw, db.
  * dresidual may be the same buffer as dsum. Workspace: cgpt_layernorm_backward_workspace_bytes(rows, hidden). */
 int cgpt_dropout_add_layernorm_forward(void* y, void* sum, const void* x, const void* residual, const void* w, const void* b,

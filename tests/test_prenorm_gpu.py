@@ -351,6 +351,46 @@ def test_fused_odd_rows_through_refilled_stages(ops, state, rows, hidden, dt):
     fused_against_its_parts_and_64_bits(ops, state, rows, hidden, dt)
 
 
+@pytest.mark.parametrize("rows,hidden,dt", [(5, 1024, "bf16"), (300, 2048, "f16"), (3, 520, "bf16"), (700, 256, "f32"), (4, 99, "bf16"), (2, 40000, "f16")])
+def test_fused_misaligned_tensors(ops, state, rows, hidden, dt):
+    """All tensors off the 16-byte grid, each by its own: the bits of the parts, and the 64-bit forms. Then only x, or only the
+    residual: sum is the same; y and the gradients are right, if not to the bit (rows are added in another order)."""
+    inputs = norm_inputs(rows, hidden, dt)
+    o, (X, W, B, DY, RES) = ops.DropoutOptions(0.2, 6), map(host, inputs)
+    x, w, b, dy, res = (shifted(a, dt, k) for a, k in zip((X, W, B, DY, RES), (1, 2, 3, 5, 6)))
+    dropped = P.drop(X, 0.2, SEED, STEP, 6)
+    S = dropped + RES
+
+    def forward(x, res, w, b, shift):
+        y, total = Guarded((rows, hidden), dt, shift), Guarded((rows, hidden), dt, shift)
+        ops.dropout_add_layernorm_forward(y.t, total.t, x, res, w, b, 1e-5, state, options=o)
+        close(total.check(), S, P.rounding(S, TORCH[dt]) + 4 * P.U * (np.abs(dropped) + np.abs(S)), "sum")
+        v = P.layernorm(host(total.t), W, B, 1e-5)
+        close(y.check(), v, P.rounding(v, TORCH[dt]) + 2 * P.layernorm_error(host(total.t), W, B, 1e-5), "y")
+        return y.t, total.t
+
+    y, total = forward(x, res, w, b, 1)
+    want_sum, want_y = Guarded(x.shape, dt, 1), Guarded(x.shape, dt, 1)
+    ops.dropout_forward(want_sum.t, x, state, options=o, residual=res)
+    ops.layernorm_forward(want_y.t, want_sum.t, w, b, 1e-5)
+    assert torch.equal(total, want_sum.t) and torch.equal(y, want_y.t)
+    for mixed in ((x, inputs[4]), (inputs[0], res)):
+        assert torch.equal(forward(*mixed, inputs[1], inputs[2], 0)[1], total)
+
+    T = host(total)
+    d, err = P.layernorm_backward(DY, T, W, 1e-5), P.layernorm_backward_error(DY, T, W, 1e-5)
+    v, e = d[0] + RES, 2 * err[0] + 2 * P.U * (np.abs(RES) + np.abs(d[0] + RES))
+    dropped = P.drop(v, 0.2, SEED, STEP, 6)
+    aligned = total.clone()
+    for shift, dy_, dsum, total_, w_ in ((1, dy, res, total, w), (0, inputs[3], res, aligned, inputs[1]), (0, dy, inputs[4], aligned, inputs[1])):
+        dx, dr, dw, db = (Guarded(s, dt, shift) for s in (x.shape, x.shape, w.shape, w.shape))
+        ops.dropout_add_layernorm_backward(dx.t, dr.t, dw.t, db.t, dy_, dsum, total_, w_, 1e-5, state, options=o)
+        close(dr.check(), v, P.rounding(v, TORCH[dt]) + e, "dresidual")
+        close(dx.check(), dropped, P.rounding(dropped, TORCH[dt]) + 1.3 * e + 3 * P.U * np.abs(dropped), "dx")
+        for got, want, bound, what in zip((dw, db), d[1:], err[1:], ("dw", "db")):
+            close(got.check(), want, P.rounding(want, TORCH[dt]) + 2 * bound, what)
+
+
 @pytest.mark.parametrize("hidden", [512, 511, 3000, 2999, 20000])
 def test_fused_in_place_sum_and_no_dropout(ops, state, hidden):
     x, w, b, _, res = norm_inputs(1200, hidden, "f16")
