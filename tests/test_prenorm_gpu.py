@@ -351,6 +351,36 @@ def test_fused_odd_rows_through_refilled_stages(ops, state, rows, hidden, dt):
     fused_against_its_parts_and_64_bits(ops, state, rows, hidden, dt)
 
 
+@pytest.mark.parametrize("rows,hidden,dt", [(120000, 64, "bf16"), (20000, 512, "f16"), (10000, 1024, "bf16"), (4000, 2056, "f16"), (700, 8192, "bf16"), (500, 12008, "f16"),
+                                            (6000, 1024, "f32"), (500, 8192, "f32")])
+def test_fused_whole_vector_rows_through_refilled_stages(ops, state, rows, hidden, dt):
+    """Every stage of the rings of both directions is filled again and used again: one, two and four vectors a lane, several rows a
+    warp, several warps a row."""
+    fused_against_its_parts_and_64_bits(ops, state, rows, hidden, dt)
+
+
+@pytest.mark.parametrize("rows,hidden,dt", [(20000, 1001, "bf16"), (56000, 250, "f16"), (11000, 1024, "bf16"), (8000, 4099, "f16"), (10000, 1001, "f32"), (2000, 8191, "bf16")])
+def test_layernorm_rows_do_not_depend_on_how_many_there_are(ops, rows, hidden, dt):
+    """A call whose rings go round more than their stages against calls of 136 rows each (a multiple of 8: every part starts on the
+    16-byte grid), which use each stage once: y has the same bits, and dx where rows are whole vectors (of other rows, the tile's
+    height says how many warps share one)."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, dy = (torch.randn(rows, hidden, device="cuda", generator=g).to(TORCH[dt]) for _ in range(2))
+    w, b = dev(1 + 0.2 * rng(0).standard_normal(hidden), dt), dev(rng(1).standard_normal(hidden), dt)
+    y, dx, dw, some = Guarded(x.shape, dt), Guarded(x.shape, dt), torch.empty_like(w), torch.empty(136, hidden, device="cuda", dtype=TORCH[dt])
+    ops.layernorm_forward(y.t, x, w, b, 1e-5)
+    ops.layernorm_backward(dx.t, dw, None, dy, x, w, 1e-5)
+    y.check(), dx.check()
+    for first in range(0, rows, 136):
+        part = slice(first, min(rows, first + 136))
+        out = some[:part.stop - first]
+        ops.layernorm_forward(out, x[part], w, b, 1e-5)
+        assert torch.equal(out, y.t[part])
+        if hidden % 8 == 0:
+            ops.layernorm_backward(out, dw, None, dy[part], x[part], w, 1e-5)
+            assert torch.equal(out, dx.t[part])
+
+
 @pytest.mark.parametrize("rows,hidden,dt", [(5, 1024, "bf16"), (300, 2048, "f16"), (3, 520, "bf16"), (700, 256, "f32"), (4, 99, "bf16"), (2, 40000, "f16")])
 def test_fused_misaligned_tensors(ops, state, rows, hidden, dt):
     """All tensors off the 16-byte grid, each by its own: the bits of the parts, and the 64-bit forms. Then only x, or only the
@@ -426,6 +456,23 @@ def test_scaled_embedding_forward(ops, state, dt, tokens, vocab, hidden):
         ops.scaled_embedding_forward(out.t, ids_dev(ids), tokens, w, state, options=ops.ScaledEmbeddingOptions(2.5, dropout=ops.DropoutOptions(p, 8)))
         want = P.drop(P.embedding(ids, host(w), 2.5), p, SEED, STEP, 8)
         close(out.check(), want, P.rounding(want, TORCH[dt]) + 4 * P.U * np.abs(want), "out")
+
+
+@pytest.mark.parametrize("hidden", [8, 40, 1024])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_scaled_embedding_forward_of_unaligned_tensors(ops, state, hidden, dt):
+    """Rows of whole vectors whose table, output or both start off the 16-byte grid: the bits of the aligned call."""
+    r = rng(hidden)
+    ids, table = r.integers(0, 60, 333).astype(np.uint32), r.standard_normal((50, hidden))
+    for p in (0.0, 0.3):
+        o, got = ops.ScaledEmbeddingOptions(2.5, dropout=ops.DropoutOptions(p, 8)), []
+        for table_shift, out_shift in ((0, 0), (1, 0), (0, 1), (3, 1)):
+            out = Guarded((333, hidden), dt, out_shift)
+            ops.scaled_embedding_forward(out.t, ids_dev(ids), 333, shifted(table, dt, table_shift), state, options=o)
+            got.append(out.check())
+        assert all(np.array_equal(got[0], g) for g in got[1:])
+        want = P.drop(P.embedding(ids, host(dev(table, dt)), 2.5), p, SEED, STEP, 8)
+        close(got[0], want, P.rounding(want, TORCH[dt]) + 4 * P.U * np.abs(want), "out")
 
 
 def backward_case(kind, tokens, vocab, r):
