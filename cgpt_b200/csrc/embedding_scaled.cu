@@ -687,7 +687,7 @@ scaled_embedding_few_kernel(T* dw, const T* __restrict__ dout, const FewArgs f, 
     __shared__ std::uint32_t present[kFewRows / 32];
     __shared__ std::uint32_t heads[kFewTokens];                         // list positions at which a row is met first
     __shared__ std::uint32_t few[kFewWarps][32];                         // per warp: the tokens it adds up
-    __shared__ int in_warp[kFewWarps], listed, rows_listed;
+    __shared__ int in_warp[kFewWarps], rows_listed;
     __shared__ __align__(16) float part[kFewWarps][32 * VEC];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const std::uint32_t shares = gridDim.x, rows = (f.vocab - blockIdx.x + shares - 1) / shares;     // row r of the CTA: r * shares + blockIdx.x

@@ -62,18 +62,12 @@ __device__ __forceinline__ void norm_sums(float (&s)[3], float dy, float w, floa
 }
 
 // Sums NV values over a warp. Halves the set of values a lane is responsible for while lanes still differ in what they hold, so
-// NV = 4 takes 6 shuffles and NV = 12 takes 18 (5 NV one value at a time). Afterwards lane l holds, in v[0 .. count), the
-// totals of the values first_of(l) .. first_of(l) + count.
+// NV = 4 takes 6 shuffles and NV = 12 takes 18 (5 NV one value at a time). Afterwards every lane holds kCount totals, in
+// v[0 .. kCount); which ones, lane bits 4 and 3 say.
 template <int NV>
 struct WarpSums {
     static constexpr int kFirst = NV % 2 == 0 ? NV / 2 : NV;
     static constexpr int kCount = NV % 4 == 0 ? NV / 4 : kFirst;
-    static __device__ __forceinline__ int first_of(int lane) {
-        int f = 0;
-        if constexpr (NV % 2 == 0) f += ((lane >> 4) & 1) * (NV / 2);
-        if constexpr (NV % 4 == 0) f += ((lane >> 3) & 1) * (NV / 4);
-        return f;
-    }
     // A lane of those that hold value i.
     static __device__ __forceinline__ constexpr int holder_of(int i) {
         int l = 0;
@@ -112,12 +106,13 @@ struct WarpSums {
     }
     // Every lane gets every total (and has it already where nothing was halved).
     static __device__ __forceinline__ void broadcast(float (&v)[NV]) {
-        if constexpr (NV % 2 != 0) return;
-        float t[NV];
+        if constexpr (NV % 2 == 0) {
+            float t[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) t[i] = __shfl_sync(0xffffffffu, v[i % kCount], holder_of(i));
+            for (int i = 0; i < NV; ++i) t[i] = __shfl_sync(0xffffffffu, v[i % kCount], holder_of(i));
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = t[i];
+            for (int i = 0; i < NV; ++i) v[i] = t[i];
+        }
     }
 };
 
@@ -517,7 +512,10 @@ int launch_backward(void* dx, void* din, void* dw, void* db, const void* dy, con
         };
         auto either = [&](auto cpt, auto cols) { return p.full ? launch(cpt, cols, std::true_type{}) : launch(cpt, cols, std::false_type{}); };
         if (p.cols == 1) return p.cpt == 1 ? either(Int<1>{}, Int<1>{}) : p.cpt == 2 ? either(Int<2>{}, Int<1>{}) : either(Int<4>{}, Int<1>{});
-        return p.cols == 2 ? either(Int<4>{}, Int<2>{}) : either(Int<4>{}, Int<4>{});
+        if (p.cols == 2) return either(Int<4>{}, Int<2>{});
+        // 16-bit rows that fill the lanes of four vectors a thread are longer than rings take
+        if constexpr (sizeof(T) == 2) return launch(Int<4>{}, Int<4>{}, std::false_type{});
+        else return either(Int<4>{}, Int<4>{});
     }
     if (form == Form::kLoose) {
         const LoosePlan p = plan_backward_loose(rows, hidden, sizeof(T));

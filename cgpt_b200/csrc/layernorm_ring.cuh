@@ -32,20 +32,19 @@ constexpr std::size_t kStatsBytes = 2 * kMaxTileRows * 32;   // static shared me
 // Rows a warp group takes at a time: a lane with few vectors per row holds several rows.
 __host__ __device__ constexpr int rows_at_once(int cpt) { return cpt >= 4 ? 1 : 4 / cpt; }
 
-// Ring of stages of consecutive rows of up to three tensors.
+// Ring of stages of consecutive rows of one tensor or two.
 struct Ring : BulkRing {
     unsigned row_bytes;
 
-    // Rows row0 .. row0 + step_rows of a, b and c (b and c may be null) into stage s, as far as there are such rows.
+    // Rows row0 .. row0 + step_rows of a and b (which may be null) into stage s, as far as there are such rows.
     template <typename T>
-    __device__ __forceinline__ void fill(int s, const T* a, const T* b, const T* c, long long row0, int step_rows, long long rows, int hidden) const {
+    __device__ __forceinline__ void fill(int s, const T* a, const T* b, long long row0, int step_rows, long long rows, int hidden) const {
         if (row0 >= rows) return;
         const unsigned n = static_cast<unsigned>(rows - row0 < step_rows ? rows - row0 : step_rows) * row_bytes;
         unsigned char* to = data + s * stage_bytes;
-        sm100::mbar_expect_tx(&full[s], (1 + (b != nullptr) + (c != nullptr)) * n);
+        sm100::mbar_expect_tx(&full[s], (1 + (b != nullptr)) * n);
         sm100::bulk_load_1d(to, a + row0 * hidden, n, &full[s]);
         if (b != nullptr) sm100::bulk_load_1d(to + tensor_bytes, b + row0 * hidden, n, &full[s]);
-        if (c != nullptr) sm100::bulk_load_1d(to + 2 * tensor_bytes, c + row0 * hidden, n, &full[s]);
     }
 };
 
@@ -144,10 +143,10 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
     ring.full = reinterpret_cast<std::uint64_t*>(shared) + group * kMaxStages;
     ring.data = shared + ra.data_offset + static_cast<std::size_t>(group) * ra.stages * ring.stage_bytes;
     ring.status = ra.status;
-    const T *second = FUSED ? residual : nullptr, *none = nullptr;
+    const T* second = FUSED ? residual : nullptr;
     if (leader) {
         ring.init();
-        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, second, none, first + s * step, ra.step_rows, rows, hidden);
+        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, second, first + s * step, ra.step_rows, rows, hidden);
     }
     stage_vector(ws, w, ra.vectors);
     stage_vector(bs, b, ra.vectors);
@@ -193,7 +192,7 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
         }
         // Every warp of the row has lifted its part of the stage (one warp: its lanes meet here).
         __syncwarp();
-        if (leader) ring.fill(ring.stage, x, second, none, row0 + ring.stages * step, ra.step_rows, rows, hidden);
+        if (leader) ring.fill(ring.stage, x, second, row0 + ring.stages * step, ra.step_rows, rows, hidden);
         ring.next();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -259,7 +258,6 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     const float inv_hidden = 1.0f / static_cast<float>(hidden);
     const long long step = static_cast<long long>(gridDim.x) * ra.step_rows;
     const long long first = static_cast<long long>(blockIdx.x) * ra.step_rows;
-    const T* none = nullptr;
     Ring ring{};
     ring.row_bytes = static_cast<unsigned>(hidden) * sizeof(T);
     ring.tensor_bytes = ra.step_rows * ring.row_bytes;
@@ -270,7 +268,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
     ring.status = ra.status;
     if (threadIdx.x == 0) {
         ring.init();
-        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, dy, none, first + s * step, ra.step_rows, rows, hidden);
+        for (int s = 0; s < ra.stages; ++s) ring.fill(s, x, dy, first + s * step, ra.step_rows, rows, hidden);
     }
     stage_vector(ws, w, ra.vectors);
     const HoistedPhilox gen(args);
@@ -384,7 +382,7 @@ layernorm_backward_ring_kernel(T* dx, T* din, float* __restrict__ partial, const
         __syncthreads();
         // Every thread is past the columns of the tile before: its stage is free.
         if (threadIdx.x == 0 && !ring.failed && row0 != first)
-            ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, none, row0 + (ring.stages - 1) * step, ra.step_rows, rows, hidden);
+            ring.fill(ring.stage == 0 ? ring.stages - 1 : ring.stage - 1, x, dy, row0 + (ring.stages - 1) * step, ra.step_rows, rows, hidden);
         // ---- columns
         auto columns = [&](auto all_rows) {
             const unsigned char* at = stage + column_bytes;
