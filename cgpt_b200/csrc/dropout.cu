@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(kThreads)
 dropout_vector_kernel(T* out, const T* in, const T* residual, long long count, const DropoutArgs args) {
     constexpr int V = 16 / sizeof(T), N = 8 / V;              // 16-byte vectors per block
     constexpr int BLOCKS = 4 / (N * (RESIDUAL ? 2 : 1));
-    const PhiloxOf<!RESIDUAL> gen(args);   // round keys kept only where nothing else is on its way
+    const PhiloxOf<RESIDUAL ? Constants::kLeft : Constants::kHoisted> gen(args);   // round keys kept only where nothing else is on its way
     const long long whole = count >> 3;
     if (blockIdx.x == 0 && threadIdx.x < (count & 7)) {       // the last elements fill no block
         const long long e = whole * 8 + threadIdx.x;

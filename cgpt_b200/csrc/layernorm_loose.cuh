@@ -142,7 +142,7 @@ layernorm_forward_loose_kernel(T* __restrict__ y, T* sum, const T* x, const T* r
     }
     stage_vector(ws, w, hidden);
     stage_vector(bs, b, hidden);
-    const Philox gen(args);
+    const KeptPhilox gen(args);
     __syncthreads();
 
     for (long long row0 = first; row0 < rows; row0 += step) {
@@ -233,7 +233,7 @@ layernorm_backward_loose_kernel(T* dx, T* din, float* __restrict__ partial, cons
         for (int s = 0; s < la.stages; ++s) ring.fill(s, x, dy, residual, first + s * step, la.step_rows, rows, hidden);
     }
     stage_vector(ws, w, hidden);
-    const Philox gen(args);
+    const KeptPhilox gen(args);
     const int row_group = K == 1 ? threadIdx.x / hidden : 0;
     const int column = K == 1 ? threadIdx.x - row_group * hidden : threadIdx.x;
     const bool works = K > 1 || row_group < la.groups;

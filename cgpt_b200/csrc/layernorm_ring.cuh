@@ -150,7 +150,7 @@ layernorm_forward_ring_kernel(T* __restrict__ y, T* sum, const T* x, const T* re
     }
     stage_vector(ws, w, ra.vectors);
     stage_vector(bs, b, ra.vectors);
-    const Philox gen(args);
+    const std::conditional_t<CPT == 8, KeptPhilox, Philox> gen(args);
     const unsigned lane_bytes = lane_row * ring.row_bytes + vec0 * 16, next_row = per_warp * ring.row_bytes;
     __syncthreads();
 

@@ -30,10 +30,18 @@ struct DropoutArgs {
 
 // The generator of one call. Of a block's counter only the first word differs within a call, so half of the first two rounds is
 // the same for all blocks and worked out once: of the second word's product in round 1 and the first word's in round 2 only what
-// the later rounds XOR in is kept, with the round keys (fused backward 74.7 -> 72.3 us, lookup 28.0 -> 27.0). HOIST: the other
-// round keys are kept in registers too, which saves their additions where registers are free.
-template <bool HOIST>
+// the later rounds XOR in is kept, with the round keys (fused backward 32768 x 1024 2.5 us less of 74, lookup of as many 1 of 28).
+//
+// What a call's constants take in registers is chosen by kernel. kLeft: the compiler works them out again where registers are short.
+// kKept: it may not. At every block the two products and their loads cost more than the registers: fused odd rows 128 | 152 us
+// forward (32768 x 1001 bf16) and 225 | 246 backward (8192 x 4099 fp16), fused forward of 4096 x 8192 bf16 56 | 62. The fused
+// forward of up to four vectors a lane has better use for them (32768 x 1024 fp16 51.6 | 50.3). kHoisted: the keys of all rounds
+// are kept as well, which saves their additions where registers are free; then the constants are left (lookup 24.6 | 23.8 us).
+enum class Constants { kLeft, kKept, kHoisted };
+
+template <Constants C>
 struct PhiloxOf {
+    static constexpr bool HOIST = C == Constants::kHoisted;
     static constexpr std::uint32_t kMul0 = 0xD2511F53u, kMul1 = 0xCD9E8D57u, kKey0 = 0x9E3779B9u, kKey1 = 0xBB67AE85u;
     std::uint32_t z1, x2, z2, z3;                                    // what rounds 1 to 3 XOR into words 2, 0, 2 and 2
     std::uint32_t k0[HOIST ? 8 : 1], k1[HOIST ? 8 : 1];              // keys of rounds 3 and later (k1[0] is in z3)
@@ -49,6 +57,7 @@ struct PhiloxOf {
         z3 = static_cast<std::uint32_t>(p) ^ (s1 + 2 * kKey1);
         k0[0] = s0 + 2 * kKey0;
         k1[0] = s1 + 2 * kKey1;
+        if constexpr (C == Constants::kKept) asm volatile("" : "+r"(z1), "+r"(x2), "+r"(z2), "+r"(z3), "+r"(k0[0]), "+r"(k1[0]));
         if constexpr (HOIST) {
 #pragma unroll
             for (int r = 1; r < 8; ++r) {
@@ -81,8 +90,9 @@ struct PhiloxOf {
         return c;
     }
 };
-using Philox = PhiloxOf<false>;
-using HoistedPhilox = PhiloxOf<true>;
+using Philox = PhiloxOf<Constants::kLeft>;
+using KeptPhilox = PhiloxOf<Constants::kKept>;
+using HoistedPhilox = PhiloxOf<Constants::kHoisted>;
 
 // Decisions are made on the high half of a word (its low half may hold anything: u >= t * 2^16 exactly if its high half >= t).
 // Products by the scale are rounded by themselves (no contraction with a residual added to them), so that every kernel gives the
