@@ -14,8 +14,9 @@
 // sort fills, while gradient rows are read, was measured slower (51 against 48 us at 32768 tokens, 32000 x 1024 bf16: the hot
 // words of the bitmap cost the sort more than it saves).
 //
-// Memory-bound without dropout: backward reads dout once and writes the table once; the sort moves 16 bytes per token and pass.
-// 32768 tokens, 32000 x 1024 bf16: 48 us, with dropout 58: sort and clearing 20, the rest the sums; the decisions make the difference.
+// Backward reads dout once and writes the table once; the sort moves 16 bytes per token and pass.
+// 32768 tokens, 32000 x 1024 bf16: 47 us, with dropout 58: sort and clearing 20, the rest the sums, in which the decisions make the
+// difference. Added to the table 45 and 57 (nothing is cleared, rows are read). 131072 tokens, sorted by launches per digit: 160 us.
 #include <algorithm>
 #include <atomic>
 
@@ -42,9 +43,9 @@ constexpr int kClusterThreads = 1024;
 constexpr int kMaxCluster = 16;
 constexpr int kMostKeys = 4;         // keys per thread of the cluster sort
 
-// kLookups consecutive tokens per group of 2^shift threads and trip: their ids, then their rows, are loaded together. What
-// bounds this kernel with dropout is the decisions (15 instructions an element, the integer pipe busy for 61 % of the time), made
-// while rows are on their way: 32768 tokens of 32000 x 1024 bf16 take 27.0 us, 3.2 TB/s of what has to move; 18.4 without dropout.
+// kLookups consecutive tokens per group of 2^shift threads and trip: their ids, then their rows, are loaded together. 32768 tokens of
+// 32000 x 1024 bf16 take 27.2 us, 3.1 TB/s of what has to move; 18.4 without dropout. No unit is full (integer pipe 61 %, 0.60
+// instructions per scheduler and cycle): ids, rows, the decisions (15 instructions an element) and stores of a trip follow one another.
 constexpr int kLookups = 4;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
@@ -257,7 +258,8 @@ sort_scatter_kernel(const SortPass p) {
 
 // The whole sort in one launch, for up to kMaxCluster * kClusterThreads * KEYS tokens: the CTAs of one cluster hold a share of the
 // keys each. Digit counts and, between passes, keys go round in distributed shared memory; only the last pass writes to global
-// memory. A pass is then two cluster barriers instead of three launches. The other clusters of the launch clear memory.
+// memory. A pass is then two cluster barriers instead of three launches. The other clusters of the launch clear memory. (Four keys a
+// thread spill 32 bytes.)
 struct ClusterSort {
     uint4* clear;                       // memory that the other clusters set to zero
     long long clear_vectors;            // 16-byte vectors of it; `clear_tail` bytes more behind them
@@ -450,7 +452,8 @@ __device__ __forceinline__ void add_floats(float (&v)[VEC], const float* from) {
     }
 }
 
-// g.groups chunks of g.chunk sorted tokens per CTA.
+// g.groups chunks of g.chunk sorted tokens per CTA. Two CTAs per SM leave 64 registers, of which the round keys take 16: 16-bit vectors
+// spill 48 bytes a thread.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kSumThreads, 2)
 scaled_embedding_sum_kernel(T* dw, const T* __restrict__ dout, const GradArgs g, const DropoutArgs args) {
@@ -624,7 +627,8 @@ scaled_embedding_join_kernel(T* dw, const GradArgs g) {
 // vectors, 4 MB table: 1 token f32 1024 wide 8 | 12; 128 tokens f32 256 wide 10 | 14; 512 tokens bf16 1024 wide 17 | 19, f32
 // 768 wide 16 | 21; 1024 tokens 22 | 18; 512 tokens and 8 MB 20 | 19; 32 MB 34 | 21 (rows cleared one by one).
 // Single elements, 513 wide: 1024 tokens f32 4 MB 23 | 33, bf16 16 MB 27 | 33; 1 token, 16 MB 12 | 16. Vectors do best with
-// a warp's width of columns per CTA (four: 33 instead of 27 for 1024 wide), single elements with four.
+// a warp's width of columns per CTA (four: 33 instead of 27 for 1024 wide), single elements with four. The rule is by the table's size
+// also where the gradient is added and nothing is cleared. Single elements of 16 bits spill 32 bytes a thread.
 constexpr int kFewTokens = 1024, kFewOfRow = 16, kFewThreads = 512, kFewWarps = kFewThreads / 32;
 constexpr unsigned kFewRows = 16384;     // rows of a CTA at most (a bit each)
 static_assert(kFewOfRow <= 32, "a warp lists 32 tokens at a time");

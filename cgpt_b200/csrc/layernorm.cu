@@ -117,7 +117,9 @@ struct WarpSums {
 };
 
 // ------------------------------------------------------------------------------------------ rows of any length
-// One CTA per row, the row read again (from L1/L2) for every pass over it. Any H, any alignment.
+// One CTA per row, the row read again (from L1/L2) for every pass over it. Any H, any alignment. Element by element, and fused a
+// generator block for every element: 4096 x 16384 bf16 takes 141 us forward, 406 backward, 372 and 617 fused, 3.4 to 6.5 times the
+// bytes' time. These rows are longer than rings hold.
 template <typename T, bool FUSED>
 __global__ void __launch_bounds__(kThreads)
 layernorm_forward_any_kernel(T* __restrict__ y, T* sum, const T* x, const T* residual, const T* __restrict__ w,

@@ -14,10 +14,13 @@
 // columns: dx, and the running dw and db of its columns in registers). Lanes that keep both a row's values and dw and db of
 // their columns need 168 registers, and 12 warps an SM hide less: measured 62 against 57 us at 16384 x 2048 bf16.
 //
-// Measured (16-bit, device times): forward 32768 x 1024 25.9 us (5.2 TB/s, 80 % of a plain copy's rate; a copy of the same bytes
-// takes 28.7), with dropout and residual 50 (5.4 TB/s); backward 16384 x 2048 with a residual 54.8 (4.9 TB/s), 32768 x 1024 44.3 (4.5 TB/s),
-// 4096 x 8192 with a residual 65.8 (4.1 TB/s), the fused one at 32768 x 1024 72.3 (4.6 TB/s: bound by instructions, the
-// decisions among them).
+// Measured (16-bit, device times): forward 32768 x 1024 26.1 us (5.1 TB/s, 80 % of a plain copy's rate; a copy of the same bytes
+// takes 28.7), with dropout and residual 50.3 (5.3 TB/s), 4096 x 8192 with both 56.1 (4.8 TB/s); backward 16384 x 2048 with a residual
+// 54.8 (4.9 TB/s), 32768 x 1024 45.3 (4.4 TB/s), 4096 x 8192 with a residual 66.6 (4.0 TB/s), the fused one at 32768 x 1024 72.2
+// (4.6 TB/s). What the backward waits for is the border between its two phases: half the issue slots are empty (0.52 instructions per
+// scheduler and cycle), with one warp eligible on average. Rows of 1025 to 1752 vectors spill 300 to 326 bytes a thread (four
+// vectors of columns and of dw and db each), 2048 x 12008 takes 87 us (1.7 TB/s); rows of fewer than 32 vectors that fill no
+// power of two of lanes 22.
 #pragma once
 
 namespace ring_kernels {

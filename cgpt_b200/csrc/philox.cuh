@@ -9,8 +9,8 @@
 // ({seed, step}, two 64-bit words), so that a captured graph draws new masks when the step is advanced between replays.
 //
 // Sixteen bits a decision, not 32: a block's ten rounds (two 32x32->64 products, four XORs and two key additions each) then
-// cover 16 bytes of a 16-bit tensor. With them dropout of a bf16 tensor still runs at memory speed (98 % of a plain copy's
-// rate at 100 M elements); the operators that do more per element, or read less, are bound by this arithmetic (each says so).
+// cover 16 bytes of a 16-bit tensor. With them dropout of a bf16 tensor still runs at memory speed (32768 x 2048 with a residual:
+// 98 % of a plain copy's rate in a loop, 93 % with other work between the calls).
 #pragma once
 
 #include <cmath>
