@@ -375,10 +375,9 @@ LoosePlan plan_backward_loose(std::size_t rows, std::size_t hidden, std::size_t 
     std::size_t tile = at_most(16 * 1024 * (2 / ctas) / (hidden * elem), loose_kernels::kMaxTileRows);
     tile = at_most(tile, over(rows, kNumSMs * ctas));
     a.step_rows = static_cast<int>(tile < 1 ? 1 : tile);
-    const int warps = p.threads / 32;
+    const int warps = p.threads / 32;                          // 16 at most: 8 units of several warps, 64 floats of sums each
     a.warps_per_row = 1;
     while (a.warps_per_row * a.step_rows * 2 <= warps && static_cast<std::size_t>(a.warps_per_row) * 64 < hidden) a.warps_per_row *= 2;
-    if (warps / a.warps_per_row > 8 && a.warps_per_row > 1) a.warps_per_row = warps / 8;   // 64 floats of sums per unit
     a.data_offset = static_cast<unsigned>(loose_vectors_end(hidden, 1));
     const std::size_t room = (kSmemPerSm + 1024) / ctas - 1024 - loose_kernels::kStatsBytes - a.data_offset;
     std::size_t stage = 0;
